@@ -381,6 +381,108 @@ int adn_op_adam(float* p, const float* g, float* m, float* v, int64_t n, float a
  * this copy against the 8 TB/s datasheet figure. */
 int adn_op_copy_bench(const float* src, float* dst, int64_t n, int repeats, void* hip_stream, float* ms);
 
+/* ---- sequence operators: layer norm, short causal convolution, selective state-space scan ------------------------------
+ * The blocks of the other family of sequence models (no reference counterpart: the reference's recurrence is the LSTM): norm ->
+ * projection -> convolution + SiLU -> projection -> gated scan -> projection.  csrc/layernorm.hip, causal_conv.hip,
+ * selective_scan.hip; Python: ip_avsr_amd/custom/sequence.py.
+ *  - All pointers are device memory; work is enqueued on hip_stream, nothing synchronises, nothing is allocated (workspaces are the
+ *    caller's), so every call may be captured into a HIP graph.
+ *  - Activations are (B, T, channels) tensors of adn_dtype elements with dense channels and any frame and utterance stride (a column
+ *    range of a wider projection, a time-major array); everything else is float32.  Statistics, states and sums are held in float32,
+ *    results are rounded once.  Outputs must not overlap inputs.
+ *  - lens (int32 [B], or null: all frames): frames at and behind an utterance's length are padding -- never read, zero in every
+ *    result, absent from every sum, and a state passes them unchanged.  Values outside [0, T] are clamped.
+ *  - All sums run in a fixed order: the same bits on every run.  No frame, utterance or element count may reach 2^31 except where the
+ *    tensor's byte size says otherwise (offsets are 64-bit).
+ * The *_workspace / *_checkpoints functions return a count of floats (< 0: sizes out of range); such buffers start on 16 bytes. */
+typedef enum { ADN_DTYPE_F32 = 0, ADN_DTYPE_BF16 = 1 } adn_dtype;
+typedef struct {
+    void* data;                  /* element (b, t, c) at data[b stride_b + t stride_t + c] */
+    int64_t stride_b, stride_t;  /* in elements */
+} adn_seq;
+
+/* y = (x - mean) inv_std gamma + beta over the channels, inv_std = 1 / sqrt(var + eps); channels <= 16384.  gamma null: 1, beta
+ * null: 0.  mean and inv_std (float32 [B][T]) are results of the forward pass and inputs of the backward pass. */
+typedef struct {
+    int32_t dtype, batch, steps, channels;
+    float eps;
+    int32_t reserved;
+    const int32_t* lens;
+    adn_seq x, y;                /* y: forward */
+    const float* gamma;
+    const float* beta;
+    float* mean;
+    float* inv_std;
+    adn_seq dy, dx;              /* backward, as are the fields below */
+    float* dgamma;               /* [channels] */
+    float* dbeta;
+    float* workspace;
+    int64_t workspace_floats;
+} adn_norm_args;
+int adn_op_layer_norm_forward(const adn_norm_args* args, void* hip_stream);
+int64_t adn_op_layer_norm_workspace(int32_t batch, int32_t steps, int32_t channels);
+int adn_op_layer_norm_backward(const adn_norm_args* args, void* hip_stream);
+
+/* y[t] = act(bias + sum_k weight[k] x[t - (taps - 1) + k]) channel by channel; weight float32 [taps][channels], taps <= 8; bias null: 0.
+ * Frames before the first come from `state` ([B][taps - 1][channels] of dtype, dense; null: zeros); state_out receives the last
+ * taps - 1 frames (of state and the valid frames together) and must be another buffer. */
+typedef enum { ADN_CONV_LINEAR = 0, ADN_CONV_SILU = 1 } adn_conv_act;
+typedef struct {
+    int32_t dtype, batch, steps, channels, taps, activation /* adn_conv_act */;
+    const int32_t* lens;
+    adn_seq x, y;                /* y: forward, step */
+    const float* weight;
+    const float* bias;
+    const void* state;
+    void* state_out;             /* forward: written; step: read and moved on in place */
+    adn_seq dy, dx;              /* backward, as are the fields below */
+    float* dweight;
+    float* dbias;
+    void* dstate;                /* gradient of `state`, or null */
+    float* workspace;
+    int64_t workspace_floats;
+} adn_conv_args;
+int adn_op_causal_conv_forward(const adn_conv_args* args, void* hip_stream);
+int64_t adn_op_causal_conv_workspace(int32_t batch, int32_t steps, int32_t channels, int32_t taps);
+int adn_op_causal_conv_backward(const adn_conv_args* args, void* hip_stream);
+/* one frame (steps = 1, no lens): y[b] from state_out[b] and x[b], state_out moved on by the frame */
+int adn_op_causal_conv_step(const adn_conv_args* args, void* hip_stream);
+
+/* dt = softplus(delta + delta_bias) (softplus = 0: no softplus), h = exp(dt A) h + dt u B_t, y = sum_n h C_t + D u, y *= z sigmoid(z).
+ * A float32 [channels][states] (finite), states <= 32; b and c: (B, T, groups * states), channel d reads group d / (channels / groups);
+ * D, delta_bias float32 [channels] or null (0); z.data null: no gate; state float32 [B][channels][states] or null (zeros).
+ * Training: the forward pass fills `checkpoints`, the backward pass reads them (same sizes, same lens) instead of `state`. */
+typedef struct {
+    int32_t dtype, batch, steps, channels, states, groups, softplus, reserved;
+    const int32_t* lens;
+    adn_seq u, delta, b, c, z, y;   /* y: forward, step */
+    const float* A;
+    const float* D;
+    const float* delta_bias;
+    const float* state;
+    float* state_out;            /* forward: written, another buffer than `state`; step: read and moved on in place */
+    float* checkpoints;          /* or null: nothing kept for a backward pass */
+    int64_t checkpoint_floats;
+    float* workspace;
+    int64_t workspace_floats;
+    adn_seq dy, du, ddelta, dz;  /* backward, as are the fields below; dz only where gated */
+    const float* dlast;          /* gradient of state_out, or null */
+    void* dB;                    /* dtype, dense (B, T, groups, states) */
+    void* dC;
+    float* dA;
+    float* dD;
+    float* ddelta_bias;
+    float* dstate;               /* gradient of `state`, or null */
+} adn_scan_args;
+int64_t adn_op_selective_scan_checkpoints(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups);
+int64_t adn_op_selective_scan_workspace(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups, int32_t backward);
+int adn_op_selective_scan_forward(const adn_scan_args* args, void* hip_stream);
+int adn_op_selective_scan_backward(const adn_scan_args* args, void* hip_stream);
+/* one frame (steps = 1, no lens): state_out moved on in place */
+int adn_op_selective_scan_step(const adn_scan_args* args, void* hip_stream);
+/* sizeof(adn_norm_args), sizeof(adn_conv_args), sizeof(adn_scan_args), for a binding to check its declarations */
+void adn_op_abi_sizes(int32_t out[3]);
+
 /* ---- feature front-end on the GPU (reference utils/preprocessing.py) -------------------------
  * Device pointers, fp32 row-major frame matrices [sum of lengths][ld], work enqueued on hip_stream.  Utterance
  * structure is passed as int32 device vectors built from the length vector: first[t] / last[t] = index of the first /

@@ -63,6 +63,35 @@ class BatchStream(C.Structure):
     _fields_ = [("frames", C.c_void_p), ("width", C.c_int32), ("elem_bytes", C.c_int32), ("out", C.c_void_p)]
 
 
+def _seq(name):
+    """The three fields of an adn_seq, flattened: a binding that fills many of them per call initialises one flat structure."""
+    return [(name, C.c_void_p), (name + "_stride_b", C.c_int64), (name + "_stride_t", C.c_int64)]
+
+
+def _pointers(*names):
+    return [(n, C.c_void_p) for n in names]
+
+
+class NormArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "steps", "channels")] + [("eps", C.c_float), ("reserved", C.c_int32)]
+                + _pointers("lens") + _seq("x") + _seq("y") + _pointers("gamma", "beta", "mean", "inv_std") + _seq("dy") + _seq("dx")
+                + _pointers("dgamma", "dbeta", "workspace") + [("workspace_floats", C.c_int64)])
+
+
+class ConvArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "steps", "channels", "taps", "activation")] + _pointers("lens") + _seq("x") + _seq("y")
+                + _pointers("weight", "bias", "state", "state_out") + _seq("dy") + _seq("dx")
+                + _pointers("dweight", "dbias", "dstate", "workspace") + [("workspace_floats", C.c_int64)])
+
+
+class ScanArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "steps", "channels", "states", "groups", "softplus", "reserved")] + _pointers("lens")
+                + _seq("u") + _seq("delta") + _seq("b") + _seq("c") + _seq("z") + _seq("y")
+                + _pointers("A", "D", "delta_bias", "state", "state_out", "checkpoints") + [("checkpoint_floats", C.c_int64)]
+                + _pointers("workspace") + [("workspace_floats", C.c_int64)] + _seq("dy") + _seq("du") + _seq("ddelta") + _seq("dz")
+                + _pointers("dlast", "dB", "dC", "dA", "dD", "ddelta_bias", "dstate"))
+
+
 class ProfileEntry(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches", C.c_int64), ("ms", C.c_double), ("flops", C.c_double),
                 ("bytes", C.c_double)]
@@ -135,6 +164,19 @@ _SIGNATURES = {
     "adn_op_delta_backward": (C.c_int, [_P, C.c_int, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
     "adn_op_adam": (C.c_int, [_P, _P, _P, _P, C.c_int64, C.c_float, _P]),
     "adn_op_copy_bench": (C.c_int, [_P, _P, C.c_int64, C.c_int, _P, C.POINTER(C.c_float)]),
+    "adn_op_abi_sizes": (None, [C.POINTER(C.c_int32)]),
+    "adn_op_layer_norm_forward": (C.c_int, [C.POINTER(NormArgs), _P]),
+    "adn_op_layer_norm_workspace": (C.c_int64, [C.c_int32] * 3),
+    "adn_op_layer_norm_backward": (C.c_int, [C.POINTER(NormArgs), _P]),
+    "adn_op_causal_conv_forward": (C.c_int, [C.POINTER(ConvArgs), _P]),
+    "adn_op_causal_conv_workspace": (C.c_int64, [C.c_int32] * 4),
+    "adn_op_causal_conv_backward": (C.c_int, [C.POINTER(ConvArgs), _P]),
+    "adn_op_causal_conv_step": (C.c_int, [C.POINTER(ConvArgs), _P]),
+    "adn_op_selective_scan_checkpoints": (C.c_int64, [C.c_int32] * 5),
+    "adn_op_selective_scan_workspace": (C.c_int64, [C.c_int32] * 6),
+    "adn_op_selective_scan_forward": (C.c_int, [C.POINTER(ScanArgs), _P]),
+    "adn_op_selective_scan_backward": (C.c_int, [C.POINTER(ScanArgs), _P]),
+    "adn_op_selective_scan_step": (C.c_int, [C.POINTER(ScanArgs), _P]),
     "adn_set_dropout_state": (C.c_int, [_P, C.c_uint32, C.c_uint32]),
     "adn_apply_sgd": (C.c_int, [_P, C.c_float, C.c_float, C.c_int]),
     "adn_apply_adadelta": (C.c_int, [_P, C.c_float, C.c_float, C.c_float]),

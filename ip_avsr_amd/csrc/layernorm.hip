@@ -1,0 +1,342 @@
+// Layer norm over the channels of a (B, T, D) tensor, forward and backward (float32 or bfloat16 rows, float32 everything else).
+//
+//   mean = E[x],  inv = 1 / sqrt(E[(x - mean)^2] + eps),  xhat = (x - mean) inv,  y = xhat gamma + beta
+//   g = dy gamma:  dx = inv (g - E[g] - xhat E[g xhat]),  dgamma = sum over rows of dy xhat,  dbeta = sum of dy
+//
+// Bound: HBM, one read of x (and dy) and one write of y (dx).  A row lives in registers from its load to its store -- the mean first,
+// then the centred second moment, so nothing cancels -- spread over 64, 256 or 1024 threads (the fewest that keep it to 16 values
+// per thread: more registers per thread cost the waves that hide the loads).  The workgroups are persistent: gamma and beta stay in
+// registers over all their rows, and the backward pass adds dgamma / dbeta there too, leaves one partial row per workgroup, and a
+// second launch adds those in a fixed order -- the same bits on every run.
+// Frames at and behind lens[b] are padding: not read, zero in every result, absent from the sums.
+#include "seq_common.h"
+
+namespace adn {
+namespace seq {
+
+namespace {
+
+struct NormParams {
+    const int32_t* lens;
+    const float* gamma;
+    const float* beta;
+    float* mean;
+    float* inv_std;
+    float* part;          // backward: [gridDim.x][2][D]
+    int T, D, rows;
+    float eps;
+};
+
+// sums of K values over the threads of a row
+template <int TPR, int K> __device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[k * NW + (threadIdx.x >> 6)] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float a = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) a += red[k * NW + w];
+            v[k] = a;
+        }
+    }
+}
+
+// thread l of a row holds columns (i TPR + l) V + j, i < NV, j < V
+template <typename T, int V, int NV, int TPR>
+__global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_forward_kernel(View<const T> x, View<T> y, NormParams p) {
+    constexpr int RPB = TPR == 1024 ? 1 : 256 / TPR;
+    __shared__ float red[2][TPR > 64 ? TPR / 64 : 1];       // mean and moment apart: a wave may be a reduction ahead of another
+    const int l = threadIdx.x % TPR;
+    float gm[NV][V], bt[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (i * TPR + l) * V + j;
+            gm[i][j] = p.gamma && c < p.D ? p.gamma[c] : 1.f;
+            bt[i][j] = p.beta && c < p.D ? p.beta[c] : 0.f;
+        }
+    const float inv_d = 1.f / (float)p.D;
+    for (int r = blockIdx.x * RPB + threadIdx.x / TPR; r < p.rows; r += gridDim.x * RPB) {
+        const int b = r / p.T, t = r - b * p.T;
+        T* yr = y.row(b, t);
+        if (t >= valid_steps(p.lens, b, p.T)) {
+            const float zero[V] = {};
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if ((i * TPR + l) * V < p.D) store_vec<T, V>(yr + (i * TPR + l) * V, zero);
+            if (l == 0) { p.mean[r] = 0.f; p.inv_std[r] = 0.f; }
+            continue;
+        }
+        const T* xr = x.row(b, t);
+        float v[NV][V], s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((i * TPR + l) * V < p.D) load_vec<T, V>(xr + (i * TPR + l) * V, v[i]);
+            else
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[0] += v[i][j];
+        row_sums<TPR, 1>(s, red[0]);
+        const float mean = s[0] * inv_d;
+        float q[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = (i * TPR + l) * V + j < p.D ? v[i][j] - mean : 0.f;
+                v[i][j] = d;
+                q[0] += d * d;
+            }
+        row_sums<TPR, 1>(q, red[1]);
+        const float inv = 1.f / sqrtf(q[0] * inv_d + p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = v[i][j] * inv * gm[i][j] + bt[i][j];
+            if ((i * TPR + l) * V < p.D) store_vec<T, V>(yr + (i * TPR + l) * V, o);
+        }
+        if (l == 0) { p.mean[r] = mean; p.inv_std[r] = inv; }
+    }
+}
+
+template <typename T, int V, int NV, int TPR>
+__global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_backward_kernel(View<const T> x, View<const T> dy, View<T> dx, NormParams p) {
+    constexpr int RPB = TPR == 1024 ? 1 : 256 / TPR;
+    constexpr int NW = TPR > 64 ? TPR / 64 : 1;
+    __shared__ float red[2][2 * NW];                         // alternating rows: one barrier per row is then enough
+    __shared__ float comb[TPR == 64 ? 2 * 64 * NV * V : 1];
+    const int l = threadIdx.x % TPR;
+    float gm[NV][V], dg[NV][V], db[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (i * TPR + l) * V + j;
+            gm[i][j] = p.gamma && c < p.D ? p.gamma[c] : 1.f;
+            dg[i][j] = 0.f;
+            db[i][j] = 0.f;
+        }
+    const float inv_d = 1.f / (float)p.D;
+    int turn = 0;
+    for (int r = blockIdx.x * RPB + threadIdx.x / TPR; r < p.rows; r += gridDim.x * RPB) {
+        const int b = r / p.T, t = r - b * p.T;
+        T* dxr = dx.row(b, t);
+        if (t >= valid_steps(p.lens, b, p.T)) {
+            const float zero[V] = {};
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if ((i * TPR + l) * V < p.D) store_vec<T, V>(dxr + (i * TPR + l) * V, zero);
+            continue;
+        }
+        const T* xr = x.row(b, t);
+        const T* gr = dy.row(b, t);
+        const float mean = p.mean[r], inv = p.inv_std[r];
+        float xh[NV][V], g[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((i * TPR + l) * V < p.D) {
+                load_vec<T, V>(xr + (i * TPR + l) * V, xh[i]);
+                load_vec<T, V>(gr + (i * TPR + l) * V, g[i]);
+            } else
+#pragma unroll
+                for (int j = 0; j < V; ++j) { xh[i][j] = mean; g[i][j] = 0.f; }
+        }
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                xh[i][j] = (xh[i][j] - mean) * inv;
+                db[i][j] += g[i][j];
+                dg[i][j] += g[i][j] * xh[i][j];
+                g[i][j] *= gm[i][j];
+                s[0] += g[i][j];
+                s[1] += g[i][j] * xh[i][j];
+            }
+        row_sums<TPR, 2>(s, red[turn]);
+        turn ^= 1;
+        const float c0 = s[0] * inv_d, c1 = s[1] * inv_d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = inv * (g[i][j] - c0 - xh[i][j] * c1);
+            if ((i * TPR + l) * V < p.D) store_vec<T, V>(dxr + (i * TPR + l) * V, o);
+        }
+    }
+    // the workgroup's partial row: rows of 64 threads add theirs wave after wave
+    float* out = p.part + (int64_t)blockIdx.x * 2 * p.D;
+    if constexpr (TPR == 64) {
+        for (int w = 0; w < RPB; ++w) {
+            if ((int)threadIdx.x / 64 == w) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = (i * 64 + l) * V + j;
+                        comb[c] = (w ? comb[c] : 0.f) + dg[i][j];
+                        comb[64 * NV * V + c] = (w ? comb[64 * NV * V + c] : 0.f) + db[i][j];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < p.D; c += 256) { out[c] = comb[c]; out[p.D + c] = comb[64 * NV * V + c]; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = (i * TPR + l) * V + j;
+                if (c < p.D) { out[c] = dg[i][j]; out[p.D + c] = db[i][j]; }
+            }
+    }
+}
+
+// 32 columns x 32 row lanes: row lane k adds parts k, k + 32, ... and the 32 sums are added in order
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict__ ws, int64_t stride, int parts, SumSegs segs, int64_t total) {
+    __shared__ float red[32][33];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + cl;
+    float a = 0.f;
+    if (c < total)
+        for (int k = rl; k < parts; k += 32) a += ws[(int64_t)k * stride + c];
+    red[rl][cl] = a;
+    __syncthreads();
+    if (rl == 0 && c < total) {
+        a = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) a += red[k][cl];
+        int64_t o = c;
+        for (int k = 0; k < segs.count; ++k) {
+            if (o < segs.n[k]) {
+                if (segs.out[k]) segs.out[k][o] = a;
+                break;
+            }
+            o -= segs.n[k];
+        }
+    }
+}
+
+constexpr int kMaxNormChannels = 16 * 1024;
+
+// backward: how many workgroups leave a partial row.  Two per CU hide each other's waits; more only add partial rows to sum
+int norm_parts(int64_t rows, int rows_per_block) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, 1024)); }
+int norm_tpr(int D) { return D <= 16 * 64 ? 64 : (D <= 16 * 256 ? 256 : 1024); }
+
+int check(const adn_norm_args* a, bool backward, const char* who) {
+    ADN_CHECK(a, ADN_ERR_INVALID, std::string(who) + ": null arguments");
+    ADN_CHECK(a->dtype == ADN_DTYPE_F32 || a->dtype == ADN_DTYPE_BF16, ADN_ERR_INVALID, std::string(who) + ": dtype is ADN_DTYPE_F32 or ADN_DTYPE_BF16");
+    ADN_CHECK(a->batch >= 0 && a->steps >= 0 && (int64_t)a->batch * a->steps < ((int64_t)1 << 31) - 65536, ADN_ERR_INVALID, std::string(who) + ": bad (batch, steps)");
+    ADN_CHECK(a->channels >= 1 && a->channels <= kMaxNormChannels, ADN_ERR_INVALID, std::string(who) + ": channels outside 1 .. 16384");
+    if (!backward) ADN_CHECK(a->eps >= 0.f, ADN_ERR_INVALID, std::string(who) + ": eps < 0");
+    const int e = a->dtype == ADN_DTYPE_BF16 ? 2 : 4;
+    if ((int64_t)a->batch * a->steps > 0) {
+        ADN_CHECK(a->mean && a->inv_std, ADN_ERR_INVALID, std::string(who) + ": null statistics");
+        ADN_CHECK(seq_ok(a->x, e) && (backward ? seq_ok(a->dy, e) && seq_ok(a->dx, e) : seq_ok(a->y, e)), ADN_ERR_INVALID,
+                  std::string(who) + ": null or misaligned tensor");
+    }
+    return ADN_OK;
+}
+
+// dispatch over element type, vector width and threads per row
+template <typename T, int V, bool BWD> int launch(const adn_norm_args& a, const NormParams& p, hipStream_t s) {
+    const int tpr = norm_tpr(p.D);
+    const int rpb = tpr == 64 ? 4 : 1;
+    const int grid = BWD ? norm_parts(p.rows, rpb) : (int)std::min<int64_t>(((int64_t)p.rows + rpb - 1) / rpb, 4096);
+    const View<const T> x = cview<T>(a.x);
+    auto go = [&](auto fwd, auto bwd, int threads) {
+        if constexpr (BWD) hipLaunchKernelGGL(bwd, dim3(grid), dim3(threads), 0, s, x, cview<T>(a.dy), view<T>(a.dx), p);
+        else hipLaunchKernelGGL(fwd, dim3(grid), dim3(threads), 0, s, x, view<T>(a.y), p);
+    };
+    constexpr int NV = 16 / V;
+#define ADN_LN_GO(TPR_, NV_) go(ln_forward_kernel<T, V, NV_, TPR_>, ln_backward_kernel<T, V, NV_, TPR_>, TPR_ == 1024 ? 1024 : 256)
+    if (tpr == 64) {
+        if (p.D <= 64 * V) ADN_LN_GO(64, 1);
+        else if (p.D <= 64 * 8) ADN_LN_GO(64, (8 / V));
+        else ADN_LN_GO(64, NV);
+    } else if (tpr == 256) {
+        if (p.D <= 256 * 8) ADN_LN_GO(256, (8 / V));
+        else ADN_LN_GO(256, NV);
+    } else {
+        if (p.D <= 1024 * 8) ADN_LN_GO(1024, (8 / V));
+        else ADN_LN_GO(1024, NV);
+    }
+#undef ADN_LN_GO
+    ADN_HIP_CHECK(hipGetLastError());
+    return ADN_OK;
+}
+
+template <bool BWD> int run(const adn_norm_args& a, const NormParams& p, hipStream_t s) {
+    const bool bf = a.dtype == ADN_DTYPE_BF16;
+    const int e = bf ? 2 : 4;
+    const bool al = a.channels * e % 16 == 0 && seq_aligned(a.x, e, 16) && (BWD ? seq_aligned(a.dy, e, 16) && seq_aligned(a.dx, e, 16) : seq_aligned(a.y, e, 16));
+    if (bf) return al ? launch<__bf16, 8, BWD>(a, p, s) : launch<__bf16, 1, BWD>(a, p, s);
+    return al ? launch<float, 4, BWD>(a, p, s) : launch<float, 1, BWD>(a, p, s);
+}
+
+NormParams params(const adn_norm_args& a) {
+    return NormParams{a.lens, a.gamma, a.beta, a.mean, a.inv_std, nullptr, a.steps, a.channels, a.batch * a.steps, a.eps};
+}
+
+}  // namespace
+
+int sum_parts(const float* ws, int64_t stride, int parts, const SumSegs& segs, hipStream_t s) {
+    int64_t total = 0;
+    for (int k = 0; k < segs.count; ++k) total += segs.n[k];
+    if (total <= 0) return ADN_OK;
+    ADN_CHECK((total + 31) / 32 < (int64_t)1 << 31, ADN_ERR_INVALID, "sum_parts: too many columns");
+    hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)((total + 31) / 32)), dim3(1024), 0, s, ws, stride, parts, segs, total);
+    ADN_HIP_CHECK(hipGetLastError());
+    return ADN_OK;
+}
+
+}  // namespace seq
+}  // namespace adn
+
+using namespace adn;
+using namespace adn::seq;
+
+extern "C" void adn_op_abi_sizes(int32_t out[3]) {
+    out[0] = (int32_t)sizeof(adn_norm_args);
+    out[1] = (int32_t)sizeof(adn_conv_args);
+    out[2] = (int32_t)sizeof(adn_scan_args);
+}
+
+extern "C" int64_t adn_op_layer_norm_workspace(int32_t batch, int32_t steps, int32_t channels) {
+    if (batch < 0 || steps < 0 || channels < 1 || channels > kMaxNormChannels) return -1;
+    const int64_t rows = (int64_t)batch * steps;
+    return rows ? (int64_t)norm_parts(rows, norm_tpr(channels) == 64 ? 4 : 1) * 2 * channels : 0;
+}
+
+extern "C" int adn_op_layer_norm_forward(const adn_norm_args* a, void* hip_stream) {
+    ADN_TRY(check(a, false, "adn_op_layer_norm_forward"));
+    if (a->batch == 0 || a->steps == 0) return ADN_OK;
+    return seq::run<false>(*a, params(*a), static_cast<hipStream_t>(hip_stream));
+}
+
+extern "C" int adn_op_layer_norm_backward(const adn_norm_args* a, void* hip_stream) {
+    ADN_TRY(check(a, true, "adn_op_layer_norm_backward"));
+    ADN_CHECK(a->dgamma && a->dbeta, ADN_ERR_INVALID, "adn_op_layer_norm_backward: null gradient");
+    const int64_t need = adn_op_layer_norm_workspace(a->batch, a->steps, a->channels);
+    ADN_CHECK(need == 0 || (a->workspace && a->workspace_floats >= need), ADN_ERR_INVALID,
+              "adn_op_layer_norm_backward: workspace smaller than adn_op_layer_norm_workspace() floats");
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    NormParams p = params(*a);
+    p.part = a->workspace;
+    if (need) ADN_TRY(seq::run<true>(*a, p, s));
+    SumSegs segs{{a->dgamma, a->dbeta}, {a->channels, a->channels}, 2};
+    return sum_parts(a->workspace, 2 * (int64_t)a->channels, (int)(need / (2 * (int64_t)a->channels)), segs, s);
+}

@@ -1,0 +1,699 @@
+// Selective state-space scan over a (B, T, D) tensor: every channel d drives N states with its own decays, a step size per frame and
+// input / output rows B_t, C_t shared by the channels of a group; forward, backward and the form for single frames.
+//
+//   dt = softplus(delta + delta_bias)  (or delta + delta_bias)
+//   a = exp(dt A[d, n]),  h[t, d, n] = a h[t-1, d, n] + dt u B[t, n],  y = sum_n h C[t, n] + D[d] u,  y *= z sigmoid(z) where gated
+//   back: dh[t] = dy C[t] + a[t+1] dh[t+1],  e = a h[t-1]
+//     ddt = sum_n dh A e + u sum_n dh B,  du = dt sum_n dh B + D dy,  dA = sum dh dt e,  dB = sum_d dh dt u,  dC = sum_d dy h
+//
+// Bound: the vector pipe.  A (t, d, n) costs a multiply, an exp2 (a quarter of the rate), a multiply and two fused multiply-adds
+// forward -- 8 issue slots of a plain instruction -- and about 17 backward, against 8 / N bytes of bfloat16 traffic.
+//
+// Layout: a quad of lanes owns NC channels and splits their states, lane `ng` of it NS of them, so a lane keeps NC NS states and
+// decays in registers and B_t, C_t cost it NS values each (staged through LDS as float32, once for the workgroup).  What belongs to
+// a (frame, channel) and not to a state -- the step size, the gate, all loads and stores -- is done once: the quad covers 4 / NC
+// frames x NC channels, one per lane, and hands dt and dt u round by quad_perm; a sum over the states is a transposing reduction of
+// 4 values over the quad (9 instructions) that leaves each lane the one it owns.  A workgroup is 4 waves of 16 NC channels.
+//
+// The backward pass walks segments of 8 frames from the end: from the state the forward pass kept at the segment's start it
+// recomputes a and e of the segment into registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by
+// exchanging halves (permlane swaps, row rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA,
+// dD and the bias' gradient stay in registers over all frames of a workgroup's utterances.  All sums run in a fixed order.
+// Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
+#include "seq_common.h"
+
+namespace adn {
+namespace seq {
+
+namespace {
+
+constexpr int kSeg = 8;               // frames of a segment: what the backward pass recomputes at a time
+constexpr int kMaxStates = 32;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+
+struct ScanParams {
+    const int32_t* lens;
+    const float* A;                   // [D][N]
+    const float* Dp;                  // [D] or null
+    const float* dbias;               // [D] or null
+    const float* state_in;            // [B][D][N] or null (zeros)
+    float* state_out;                 // [B][D][N]
+    float* ckpt;                      // states before every segment: [B][nseg][ctiles][P / 4][64][4], or null
+    const float* dlast;               // backward: gradient of state_out, or null
+    float* dstate;                    // backward: gradient of state_in, or null
+    float* part_bc;                   // backward: [bpg][B][nseg][G][kSeg][2][4 NS]
+    float* part_a;                    // backward: [nbg][ctiles][64 P + 2 * 16 NC]
+    int B, T, D, N, G, Dg;            // Dg = D / G channels per group
+    int nseg, tpg, bpg, ctiles;       // segments; waves and workgroups per group; waves of all workgroups along the channels
+    int nbg, per_bg;                  // backward: groups of utterances, utterances per group
+    int softplus;
+};
+
+// channels of a quad: with NS states per lane, 8 (channel, state) pairs per lane (4 where N <= 4)
+constexpr int channels_per_quad(int ns) { return ns == 8 ? 1 : (ns == 4 ? 2 : 4); }
+
+// log(1 + exp(x)), relative accuracy also where it is small: log1p(e) = 2 atanh(e / (2 + e)) of e = exp(-|x|) <= 1, whose odd series
+// in s = e / (2 + e) <= 1/3 is cut where the rest is below 2^-26 of it
+__device__ __forceinline__ float softplusf(float x) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float r = 1.f / 15.f;
+    r = fmaf(r, q, 1.f / 13.f);
+    r = fmaf(r, q, 1.f / 11.f);
+    r = fmaf(r, q, 1.f / 9.f);
+    r = fmaf(r, q, 1.f / 7.f);
+    r = fmaf(r, q, 1.f / 5.f);
+    r = fmaf(r, q, 1.f / 3.f);
+    r = fmaf(r, q, 1.f);
+    return fmaxf(x, 0.f) + 2.f * s * r;
+}
+
+__device__ __forceinline__ float bcast(float v, int q) {
+    switch (q) {
+        case 0: return quad_bcast<0>(v);
+        case 1: return quad_bcast<1>(v);
+        case 2: return quad_bcast<2>(v);
+        default: return quad_bcast<3>(v);
+    }
+}
+// lane ng of a quad: the sum over the quad of v[ng]
+__device__ __forceinline__ float quad_gather(const float (&v)[4], bool b0, bool b1) {
+    const float x0 = (b0 ? v[1] : v[0]) + dpp<kQuadXor1>(b0 ? v[0] : v[1]);
+    const float x1 = (b0 ? v[3] : v[2]) + dpp<kQuadXor1>(b0 ? v[2] : v[3]);
+    return (b1 ? x1 : x0) + dpp<kQuadXor2>(b1 ? x0 : x1);
+}
+
+// where a wave and its lanes stand
+template <int NS, int NC> struct Place {
+    static constexpr int TQ = 4 / NC, WC = 16 * NC, P = NC * NS, Q = kSeg / TQ;
+    int lane, wv, ng, cl, g, ctile, c0, cend, oc, otp;
+    bool ocv, b0, b1;
+    __device__ __forceinline__ Place(const ScanParams& p, int cblk) {
+        lane = threadIdx.x & 63;
+        wv = threadIdx.x / 64;
+        ng = lane & 3;
+        cl = lane >> 2;
+        g = cblk / p.bpg;
+        const int tg = (cblk - g * p.bpg) * 4 + wv;
+        ctile = cblk * 4 + wv;
+        c0 = g * p.Dg + tg * WC + cl * NC;          // the quad's first channel
+        cend = (g + 1) * p.Dg;
+        oc = c0 + ng % NC;                          // the channel and, below, the frame of the quad that this lane owns
+        otp = ng / NC;
+        ocv = oc < cend;
+        b0 = ng & 1;
+        b1 = ng >> 1;
+    }
+};
+
+// B and C rows of a segment: value i of kSeg x 2 x 4 NS; 0 behind the length and behind N
+template <typename T, int NS>
+__device__ __forceinline__ float stage_value(const View<const T>& bm, const View<const T>& cm, const ScanParams& p, int b, int g, int t0, int len, int i) {
+    const int s = i / (8 * NS), n = i % (4 * NS), t = t0 + s;
+    if (s >= kSeg || t >= len || t < 0 || n >= p.N) return 0.f;
+    return (float)((i / (4 * NS)) & 1 ? cm : bm).row(b, t)[(int64_t)g * p.N + n];
+}
+
+template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p, int b, int seg, int ctile, int lane) {
+    return (((int64_t)b * p.nseg + seg) * p.ctiles + ctile) * 64 * P + lane * 4;
+}
+
+template <typename T, int NS, int NC, bool GATED, bool SAVE>
+__global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
+                                                           View<T> y, ScanParams p) {
+    using L = Place<NS, NC>;
+    constexpr int TQ = L::TQ, P = L::P, Q = L::Q, STAGE = kSeg * 8 * NS, SPT = (STAGE + 255) / 256;
+    __shared__ __align__(16) float bc[2][STAGE];
+    const int cb = p.bpg * p.G;
+    const int b = (int)(blockIdx.x / cb);
+    const L l(p, (int)(blockIdx.x - (unsigned)b * cb));
+    const int len = valid_steps(p.lens, b, p.T), nv = (len + kSeg - 1) / kSeg;
+    float A2[NC][NS], h[NC][NS];
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int c = l.c0 + k, n = l.ng * NS + j;
+            const bool on = c < l.cend && n < p.N;
+            A2[k][j] = on ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            h[k][j] = on && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+        }
+    const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
+    T un[Q], xn[Q], zn[Q];
+    float st[SPT];
+    auto fetch = [&](int seg) {
+        const int t0 = seg * kSeg;
+#pragma unroll
+        for (int m = 0; m < SPT; ++m) st[m] = stage_value<T, NS>(bm, cm, p, b, l.g, t0, len, threadIdx.x + 256 * m);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int t = t0 + i * TQ + l.otp;
+            const bool on = l.ocv && t < len;
+            un[i] = on ? u.row(b, t)[l.oc] : (T)0.f;
+            xn[i] = on ? delta.row(b, t)[l.oc] : (T)0.f;
+            if (GATED) zn[i] = on ? z.row(b, t)[l.oc] : (T)0.f;
+        }
+    };
+    if (nv) fetch(0);
+    for (int seg = 0; seg < nv; ++seg) {
+        float* buf = bc[seg & 1];
+#pragma unroll
+        for (int m = 0; m < SPT; ++m)
+            if ((int)threadIdx.x + 256 * m < STAGE) buf[threadIdx.x + 256 * m] = st[m];
+        __syncthreads();            // (the other buffer may still be read by a wave in the segment before)
+        float uc[Q], xc[Q], zc[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            uc[i] = (float)un[i];
+            xc[i] = (float)xn[i] + bias;
+            if (GATED) zc[i] = (float)zn[i];
+        }
+        if (seg + 1 < nv) fetch(seg + 1);
+        if (SAVE) {
+            float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile, l.lane);
+#pragma unroll
+            for (int m = 0; m < P / 4; ++m) {
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = h[(m * 4 + j) / NS][(m * 4 + j) % NS];
+                store_vec<float, 4>(ck + m * 256, v);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int t = seg * kSeg + i * TQ + l.otp;
+            const float dt = t < len ? (p.softplus ? softplusf(xc[i]) : xc[i]) : 0.f;      // dt = 0: the state passes a padding frame
+            const float dtu = dt * uc[i];
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int tp = 0; tp < TQ; ++tp) {
+                float bv[NS], cv[NS];
+                load_vec<float, NS>(buf + (i * TQ + tp) * 8 * NS + l.ng * NS, bv);
+                load_vec<float, NS>(buf + (i * TQ + tp) * 8 * NS + 4 * NS + l.ng * NS, cv);
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const int q = tp * NC + k;
+                    const float dtk = bcast(dt, q), dtuk = bcast(dtu, q);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const float a = __builtin_amdgcn_exp2f(dtk * A2[k][j]);
+                        h[k][j] = fmaf(a, h[k][j], dtuk * bv[j]);
+                        acc[q] = fmaf(h[k][j], cv[j], acc[q]);
+                    }
+                }
+            }
+            float o = quad_gather(acc, l.b0, l.b1) + Dv * uc[i];
+            if (GATED) o *= zc[i] * sigmoidf(zc[i]);
+            if (l.ocv && t < p.T) y.row(b, t)[l.oc] = (T)(t < len ? o : 0.f);
+        }
+    }
+    for (int t = nv * kSeg + l.otp; t < p.T; t += TQ)
+        if (l.ocv) y.row(b, t)[l.oc] = (T)0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int c = l.c0 + k, n = l.ng * NS + j;
+            if (c < l.cend && n < p.N) p.state_out[((int64_t)b * p.D + c) * p.N + n] = h[k][j];
+        }
+}
+
+// sum over the 16 quads of a wave of the 2 NS values of each lane (NS of dB, NS of dC), each sum in one lane per ng: halves are
+// exchanged while there are several values, so a step halves the values and adds one bit of the lane to the place
+template <int NS> __device__ __forceinline__ void reduce_quads(float (&v)[2 * NS], const int lane, float* out) {
+    constexpr int V = 2 * NS;
+    float r1[V / 2], r2[(V + 3) / 4];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r1[i] = add_swap32(v[i], v[i + V / 2]);
+    int at = (lane >> 5) * (V / 2);
+    if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) r2[i] = add_swap16(r1[i], r1[i + V / 4]);
+        at += ((lane >> 4) & 1) * (V / 4);
+    } else {
+        r2[0] = add_swap16(r1[0], r1[0]);
+    }
+    const bool b3 = lane & 8, b2 = lane & 4;
+    bool mine = V >= 4 || (lane & 16);
+    float r;
+    if constexpr (V >= 8) {
+        float r3[V / 8];
+#pragma unroll
+        for (int i = 0; i < V / 8; ++i) r3[i] = (b3 ? r2[i + V / 8] : r2[i]) + dpp<kRowRor8>(b3 ? r2[i] : r2[i + V / 8]);
+        at += b3 ? V / 8 : 0;
+        if constexpr (V >= 16) {
+            const float give = b2 ? r3[0] : r3[1];
+            // lane ^ 4
+            r = (b2 ? r3[1] : r3[0]) + __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, give), 0x101F));
+            at += b2 ? 1 : 0;
+        } else {
+            r = r3[0] + dpp<0x114>(r3[0]);          // row_shr:4: complete in the lanes with bit 2 set
+            mine = mine && b2;
+        }
+    } else {
+        r = r2[0] + dpp<kRowRor8>(r2[0]);
+        r = r + dpp<0x114>(r);
+        mine = mine && b2 && b3;
+    }
+    if (mine) out[(at / NS) * 4 * NS + (lane & 3) * NS + at % NS] = r;
+}
+
+template <typename T, int NS, int NC, bool GATED>
+__global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
+                                                               View<const T> dy, View<T> du, View<T> ddelta, View<T> dz, ScanParams p) {
+    using L = Place<NS, NC>;
+    constexpr int TQ = L::TQ, P = L::P, Q = L::Q, WC = L::WC, STAGE = kSeg * 8 * NS, SPT = (STAGE + 255) / 256;
+    __shared__ __align__(16) float bc[2][STAGE];
+    __shared__ float red[2][4][STAGE];
+    const int cb = p.bpg * p.G;
+    const int bg = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)bg * cb);
+    const L l(p, cblk);
+    float A2[NC][NS], dA[NC][NS];
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int c = l.c0 + k, n = l.ng * NS + j;
+            A2[k][j] = c < l.cend && n < p.N ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            dA[k][j] = 0.f;
+        }
+    const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
+    float dD = 0.f, dbias = 0.f;
+    int turn = 0;
+    int64_t flush_at = -1;                      // where the sums waiting in red[turn ^ 1] go
+    auto flush = [&](const float (*rd)[STAGE]) {
+        for (int i = threadIdx.x; i < STAGE; i += 256) p.part_bc[flush_at + i] = ((rd[0][i] + rd[1][i]) + rd[2][i]) + rd[3][i];
+    };
+    const int b_end = min(p.B, (bg + 1) * p.per_bg);
+    for (int b = bg * p.per_bg; b < b_end; ++b) {
+        const int len = valid_steps(p.lens, b, p.T), nv = (len + kSeg - 1) / kSeg;
+        float carry[NC][NS];
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const int c = l.c0 + k, n = l.ng * NS + j;
+                carry[k][j] = p.dlast && c < l.cend && n < p.N ? p.dlast[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+            }
+        for (int t = nv * kSeg + l.otp; t < p.T; t += TQ)
+            if (l.ocv) {
+                du.row(b, t)[l.oc] = (T)0.f;
+                ddelta.row(b, t)[l.oc] = (T)0.f;
+                if (GATED) dz.row(b, t)[l.oc] = (T)0.f;
+            }
+        T un[Q], xn[Q], zn[Q], gn[Q];
+        float st[SPT], hn[P];
+        auto fetch = [&](int seg) {
+            const int t0 = seg * kSeg;
+#pragma unroll
+            for (int m = 0; m < SPT; ++m) st[m] = stage_value<T, NS>(bm, cm, p, b, l.g, t0, len, threadIdx.x + 256 * m);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const int t = t0 + i * TQ + l.otp;
+                const bool on = l.ocv && t < len;
+                un[i] = on ? u.row(b, t)[l.oc] : (T)0.f;
+                xn[i] = on ? delta.row(b, t)[l.oc] : (T)0.f;
+                gn[i] = on ? dy.row(b, t)[l.oc] : (T)0.f;
+                if (GATED) zn[i] = on ? z.row(b, t)[l.oc] : (T)0.f;
+            }
+            const float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile, l.lane);
+#pragma unroll
+            for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(ck + m * 256, hn + m * 4);
+        };
+        if (nv) fetch(nv - 1);
+        for (int seg = nv - 1; seg >= 0; --seg) {
+            float* buf = bc[turn];
+#pragma unroll
+            for (int m = 0; m < SPT; ++m)
+                if ((int)threadIdx.x + 256 * m < STAGE) buf[threadIdx.x + 256 * m] = st[m];
+            __syncthreads();                    // B and C are in; the sums of the segment before are complete
+            if (flush_at >= 0) flush(red[turn ^ 1]);
+            flush_at = ((((int64_t)(cblk - l.g * p.bpg) * p.B + b) * p.nseg + seg) * p.G + l.g) * STAGE;
+            float uc[Q], xc[Q], zc[Q], gc[Q], dt[Q], h[NC][NS];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const int t = seg * kSeg + i * TQ + l.otp;
+                uc[i] = (float)un[i];
+                xc[i] = (float)xn[i] + bias;
+                gc[i] = (float)gn[i];
+                if (GATED) zc[i] = (float)zn[i];
+                dt[i] = t < len ? (p.softplus ? softplusf(xc[i]) : xc[i]) : 0.f;
+            }
+#pragma unroll
+            for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
+            if (seg > 0) fetch(seg - 1);
+            float a[kSeg][NC][NS], e[kSeg][NC][NS];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const float dtu = dt[i] * uc[i];
+#pragma unroll
+                for (int tp = 0; tp < TQ; ++tp) {
+                    const int s = i * TQ + tp;
+                    float bv[NS];
+                    load_vec<float, NS>(buf + s * 8 * NS + l.ng * NS, bv);
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        const float dtk = bcast(dt[i], tp * NC + k), dtuk = bcast(dtu, tp * NC + k);
+#pragma unroll
+                        for (int j = 0; j < NS; ++j) {
+                            a[s][k][j] = __builtin_amdgcn_exp2f(dtk * A2[k][j]);
+                            e[s][k][j] = a[s][k][j] * h[k][j];
+                            h[k][j] = fmaf(dtuk, bv[j], e[s][k][j]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = Q - 1; i >= 0; --i) {
+                const float dtu = dt[i] * uc[i];
+                float sg = 0.f, dyp = gc[i];
+                if (GATED) { sg = sigmoidf(zc[i]); dyp *= zc[i] * sg; }
+                float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f}, sy[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int tp = TQ - 1; tp >= 0; --tp) {
+                    const int s = i * TQ + tp;
+                    float bv[NS], cv[NS], sums[2 * NS];
+                    load_vec<float, NS>(buf + s * 8 * NS + l.ng * NS, bv);
+                    load_vec<float, NS>(buf + s * 8 * NS + 4 * NS + l.ng * NS, cv);
+#pragma unroll
+                    for (int j = 0; j < 2 * NS; ++j) sums[j] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) {
+                        const int q = tp * NC + k;
+                        const float dtk = bcast(dt[i], q), dtuk = bcast(dtu, q), dyk = bcast(dyp, q);
+#pragma unroll
+                        for (int j = 0; j < NS; ++j) {
+                            const float dh = fmaf(cv[j], dyk, carry[k][j]), hv = fmaf(dtuk, bv[j], e[s][k][j]), de = dh * e[s][k][j];
+                            sums[j] = fmaf(dtuk, dh, sums[j]);
+                            sums[NS + j] = fmaf(dyk, hv, sums[NS + j]);
+                            s1[q] = fmaf(dh, bv[j], s1[q]);
+                            s2[q] = fmaf(A2[k][j], de, s2[q]);
+                            if (GATED) sy[q] = fmaf(cv[j], hv, sy[q]);
+                            dA[k][j] = fmaf(dtk, de, dA[k][j]);
+                            carry[k][j] = a[s][k][j] * dh;
+                        }
+                    }
+                    reduce_quads<NS>(sums, l.lane, red[turn][l.wv] + s * 8 * NS);
+                }
+                const int t = seg * kSeg + i * TQ + l.otp;
+                const float ddtu = quad_gather(s1, l.b0, l.b1), ddec = quad_gather(s2, l.b0, l.b1) * kLn2;
+                float dx = ddec + uc[i] * ddtu;
+                if (p.softplus) dx *= sigmoidf(xc[i]);
+                if (!(t < len)) dx = 0.f;
+                const float duv = dt[i] * ddtu + Dv * dyp;
+                dbias += dx;
+                dD += dyp * uc[i];
+                if (l.ocv && t < p.T) {
+                    du.row(b, t)[l.oc] = (T)duv;
+                    ddelta.row(b, t)[l.oc] = (T)dx;
+                }
+                if (GATED) {
+                    const float yp = quad_gather(sy, l.b0, l.b1) + Dv * uc[i];
+                    if (l.ocv && t < p.T) dz.row(b, t)[l.oc] = (T)(gc[i] * yp * sg * (1.f + zc[i] * (1.f - sg)));
+                }
+            }
+            turn ^= 1;
+        }
+        if (p.dstate)
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const int c = l.c0 + k, n = l.ng * NS + j;
+                    if (c < l.cend && n < p.N) p.dstate[((int64_t)b * p.D + c) * p.N + n] = carry[k][j];
+                }
+    }
+    __syncthreads();
+    if (flush_at >= 0) flush(red[turn ^ 1]);
+    float* out = p.part_a + ((int64_t)bg * p.ctiles + l.ctile) * (64 * P + 2 * WC);
+#pragma unroll
+    for (int m = 0; m < P / 4; ++m) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = dA[(m * 4 + j) / NS][(m * 4 + j) % NS];
+        store_vec<float, 4>(out + (m * 64 + l.lane) * 4, v);
+    }
+    if constexpr (TQ == 4) { dD += dpp<kQuadXor1>(dD); dbias += dpp<kQuadXor1>(dbias); }
+    if constexpr (TQ >= 2) { dD += dpp<kQuadXor2>(dD); dbias += dpp<kQuadXor2>(dbias); }
+    if (l.otp == 0) {
+        out[64 * P + l.cl * NC + l.ng] = dD;
+        out[64 * P + WC + l.cl * NC + l.ng] = dbias;
+    }
+}
+
+// the second launch of the backward pass: workgroups [0, nb_bc) add dB and dC over the workgroups of a group, the others dA, dD and
+// the bias' gradient over the groups of utterances
+template <typename T, int NS, int NC>
+__global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T* __restrict__ dC, float* __restrict__ dA, float* __restrict__ dD,
+                                                          float* __restrict__ dbias, ScanParams p, int nb_bc) {
+    constexpr int P = NC * NS, WC = 16 * NC, STAGE = kSeg * 8 * NS;
+    if ((int)blockIdx.x < nb_bc) {
+        const int64_t gn = (int64_t)p.G * p.N, total = (int64_t)p.B * p.T * gn * 2;
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (i >= total) return;
+        const int which = i >= total / 2;
+        const int64_t o = i - (which ? total / 2 : 0), bt = o / gn;
+        const int n = (int)(o % p.N), g = (int)(o % gn) / p.N, b = (int)(bt / p.T), t = (int)(bt % p.T);
+        float a = 0.f;
+        if (t < valid_steps(p.lens, b, p.T)) {
+            const float* src = p.part_bc + (((int64_t)b * p.nseg + t / kSeg) * p.G + g) * STAGE + (t % kSeg) * 8 * NS + which * 4 * NS + n;
+            for (int k = 0; k < p.bpg; ++k) a += src[(int64_t)k * p.B * p.nseg * p.G * STAGE];
+        }
+        (which ? dC : dB)[o] = (T)a;
+        return;
+    }
+    const int64_t i = (int64_t)(blockIdx.x - nb_bc) * 256 + threadIdx.x, da = (int64_t)p.D * p.N;
+    if (i >= da + 2 * (int64_t)p.D) return;
+    const int c = (int)(i < da ? i / p.N : (i - da) % p.D), n = (int)(i % p.N);
+    const int g = c / p.Dg, cg = c - g * p.Dg, tg = cg / WC, cw = cg % WC;
+    const int64_t row = (int64_t)(g * p.bpg * 4 + tg) * (64 * P + 2 * WC), stride = (int64_t)p.ctiles * (64 * P + 2 * WC);
+    int64_t at;
+    if (i < da) {
+        const int lane = cw / NC * 4 + n / NS, m = cw % NC * NS + n % NS;
+        at = (m / 4 * 64 + lane) * 4 + m % 4;
+    } else
+        at = 64 * P + (i - da >= p.D ? WC : 0) + cw;
+    float a = 0.f;
+    for (int k = 0; k < p.nbg; ++k) a += p.part_a[row + at + k * stride];
+    if (i < da) dA[i] = a;
+    else if (i - da < p.D) dD[c] = a;
+    else dbias[c] = a;
+}
+
+// one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane
+template <typename T, int NS>
+__global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u, int64_t ldu, const T* __restrict__ delta, int64_t ldd, const T* __restrict__ bm,
+                                                        int64_t ldb, const T* __restrict__ cm, int64_t ldc, const T* __restrict__ z, int64_t ldz,
+                                                        T* __restrict__ y, int64_t ldy, ScanParams p) {
+    const int64_t item = (int64_t)blockIdx.x * 64 + threadIdx.x / 4;
+    const int ng = threadIdx.x & 3;
+    if (item >= (int64_t)p.B * p.D) return;              // whole quads leave
+    const int b = (int)(item / p.D), c = (int)(item - (int64_t)b * p.D), g = c / p.Dg;
+    const float uv = (float)u[b * ldu + c];
+    float dt = (float)delta[b * ldd + c] + (p.dbias ? p.dbias[c] : 0.f);
+    if (p.softplus) dt = softplusf(dt);
+    const float dtu = dt * uv;
+    float* h = p.state_out + item * p.N;
+    const T* br = bm + b * ldb + (int64_t)g * p.N;
+    const T* cr = cm + b * ldc + (int64_t)g * p.N;
+    float acc = 0.f;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        const int n = ng * NS + j;
+        if (n < p.N) {
+            const float a = __builtin_amdgcn_exp2f(dt * (p.A[(int64_t)c * p.N + n] * kLog2e));
+            const float hv = fmaf(a, h[n], dtu * (float)br[n]);
+            h[n] = hv;
+            acc = fmaf(hv, (float)cr[n], acc);
+        }
+    }
+    acc += dpp<kQuadXor1>(acc);
+    acc += dpp<kQuadXor2>(acc);
+    if (ng == 0) {
+        float o = acc + (p.Dp ? p.Dp[c] : 0.f) * uv;
+        if (z) {
+            const float zv = (float)z[b * ldz + c];
+            o *= zv * sigmoidf(zv);
+        }
+        y[b * ldy + c] = (T)o;
+    }
+}
+
+int states_per_lane(int n) { return n <= 4 ? 1 : (n <= 8 ? 2 : (n <= 16 ? 4 : 8)); }
+
+struct Plan { int ns, nc, nseg, tpg, bpg, ctiles, nbg, per_bg; int64_t ckpt, part_bc, part_a; };
+
+Plan plan_of(int64_t B, int64_t T, int D, int N, int G) {
+    Plan q{};
+    q.ns = states_per_lane(N);
+    q.nc = channels_per_quad(q.ns);
+    const int Dg = D / G, P = q.ns * q.nc, WC = 16 * q.nc;
+    q.nseg = cdiv(T, kSeg);
+    q.tpg = cdiv(Dg, WC);
+    q.bpg = cdiv(q.tpg, 4);
+    q.ctiles = q.bpg * G * 4;
+    q.ckpt = B * q.nseg * q.ctiles * 64 * P;
+    // backward: enough groups of utterances for two workgroups per CU
+    const int64_t want = std::max<int64_t>(1, cdiv(1024, q.bpg * G));
+    q.per_bg = (int)std::max<int64_t>(1, B / want);
+    q.nbg = cdiv(B, q.per_bg);
+    q.part_bc = (int64_t)q.bpg * B * q.nseg * G * kSeg * 8 * q.ns;
+    q.part_a = (int64_t)q.nbg * q.ctiles * (64 * P + 2 * WC);
+    return q;
+}
+
+bool sizes_ok(int64_t B, int64_t T, int64_t D, int64_t N, int64_t G) {
+    return B >= 0 && T >= 0 && B * T < ((int64_t)1 << 31) - 65536 && D >= 1 && D <= 1 << 20 && N >= 1 && N <= kMaxStates && G >= 1 && D % G == 0 &&
+           B * D < (int64_t)1 << 31;
+}
+
+int check(const adn_scan_args* a, const char* who, bool backward) {
+    ADN_CHECK(a, ADN_ERR_INVALID, std::string(who) + ": null arguments");
+    ADN_CHECK(a->dtype == ADN_DTYPE_F32 || a->dtype == ADN_DTYPE_BF16, ADN_ERR_INVALID, std::string(who) + ": dtype is ADN_DTYPE_F32 or ADN_DTYPE_BF16");
+    ADN_CHECK(a->batch >= 0 && a->steps >= 0 && (int64_t)a->batch * a->steps < ((int64_t)1 << 31) - 65536, ADN_ERR_INVALID, std::string(who) + ": bad (batch, steps)");
+    ADN_CHECK(a->states >= 1 && a->states <= kMaxStates, ADN_ERR_INVALID, std::string(who) + ": states outside 1 .. 32");
+    ADN_CHECK(a->channels >= 1 && a->channels <= 1 << 20 && a->groups >= 1 && a->channels % a->groups == 0, ADN_ERR_INVALID,
+              std::string(who) + ": channels outside 1 .. 2^20 or not a multiple of groups");
+    ADN_CHECK(sizes_ok(a->batch, a->steps, a->channels, a->states, a->groups), ADN_ERR_INVALID, std::string(who) + ": batch * channels too large");
+    ADN_CHECK(a->A, ADN_ERR_INVALID, std::string(who) + ": null A");
+    const int e = a->dtype == ADN_DTYPE_BF16 ? 2 : 4;
+    if ((int64_t)a->batch * a->steps > 0) {
+        ADN_CHECK(seq_ok(a->u, e) && seq_ok(a->delta, e) && seq_ok(a->b, e) && seq_ok(a->c, e), ADN_ERR_INVALID, std::string(who) + ": null or misaligned tensor");
+        ADN_CHECK(!a->z.data || seq_ok(a->z, e), ADN_ERR_INVALID, std::string(who) + ": misaligned gate");
+        if (!backward) ADN_CHECK(seq_ok(a->y, e), ADN_ERR_INVALID, std::string(who) + ": null or misaligned y");
+        else ADN_CHECK(seq_ok(a->dy, e) && seq_ok(a->du, e) && seq_ok(a->ddelta, e) && (!a->z.data || seq_ok(a->dz, e)), ADN_ERR_INVALID,
+                       std::string(who) + ": null or misaligned gradient");
+    }
+    return ADN_OK;
+}
+
+ScanParams params(const adn_scan_args& a, const Plan& q) {
+    ScanParams p{};
+    p.lens = a.lens; p.A = a.A; p.Dp = a.D; p.dbias = a.delta_bias; p.state_in = a.state; p.state_out = a.state_out; p.ckpt = a.checkpoints;
+    p.dlast = a.dlast; p.dstate = a.dstate;
+    p.B = a.batch; p.T = a.steps; p.D = a.channels; p.N = a.states; p.G = a.groups; p.Dg = a.channels / a.groups;
+    p.nseg = q.nseg; p.tpg = q.tpg; p.bpg = q.bpg; p.ctiles = q.ctiles; p.nbg = q.nbg; p.per_bg = q.per_bg;
+    p.softplus = a.softplus;
+    return p;
+}
+
+template <typename T, int NS> int forward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
+    constexpr int NC = channels_per_quad(NS);
+    const dim3 grid((unsigned)((int64_t)p.B * p.bpg * p.G));
+#define ADN_SCAN_GO(GATED, SAVE)                                                                                                                        \
+    hipLaunchKernelGGL((scan_forward_kernel<T, NS, NC, GATED, SAVE>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
+                       cview<T>(a.z), view<T>(a.y), p)
+    if (a.z.data) {
+        if (p.ckpt) ADN_SCAN_GO(true, true);
+        else ADN_SCAN_GO(true, false);
+    } else {
+        if (p.ckpt) ADN_SCAN_GO(false, true);
+        else ADN_SCAN_GO(false, false);
+    }
+#undef ADN_SCAN_GO
+    ADN_HIP_CHECK(hipGetLastError());
+    return ADN_OK;
+}
+
+template <typename T, int NS> int backward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
+    constexpr int NC = channels_per_quad(NS);
+    const dim3 grid((unsigned)((int64_t)p.nbg * p.bpg * p.G));
+#define ADN_SCAN_GO(GATED)                                                                                                                          \
+    hipLaunchKernelGGL((scan_backward_kernel<T, NS, NC, GATED>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
+                       cview<T>(a.z), cview<T>(a.dy), view<T>(a.du), view<T>(a.ddelta), view<T>(a.dz), p)
+    if (p.B > 0) {
+        if (a.z.data) ADN_SCAN_GO(true);
+        else ADN_SCAN_GO(false);
+        ADN_HIP_CHECK(hipGetLastError());
+    }
+#undef ADN_SCAN_GO
+    const int64_t bc = (int64_t)p.B * p.T * p.G * p.N * 2, rest = (int64_t)p.D * (p.N + 2);
+    const int64_t nb_bc = (bc + 255) / 256;
+    ADN_CHECK(nb_bc + (rest + 255) / 256 < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
+    hipLaunchKernelGGL((scan_reduce_kernel<T, NS, NC>), dim3((unsigned)(nb_bc + (rest + 255) / 256)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
+                       a.dA, a.dD, a.ddelta_bias, p, (int)nb_bc);
+    ADN_HIP_CHECK(hipGetLastError());
+    return ADN_OK;
+}
+
+template <typename T, int NS> int step(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
+    const int64_t items = (int64_t)p.B * p.D;
+    hipLaunchKernelGGL((scan_step_kernel<T, NS>), dim3((unsigned)((items + 63) / 64)), dim3(256), 0, s, static_cast<const T*>(a.u.data), a.u.stride_b,
+                       static_cast<const T*>(a.delta.data), a.delta.stride_b, static_cast<const T*>(a.b.data), a.b.stride_b, static_cast<const T*>(a.c.data),
+                       a.c.stride_b, static_cast<const T*>(a.z.data), a.z.stride_b, static_cast<T*>(a.y.data), a.y.stride_b, p);
+    ADN_HIP_CHECK(hipGetLastError());
+    return ADN_OK;
+}
+
+enum Pass { kForward, kBackward, kStep };
+template <typename T, Pass PASS, int NS> int go(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
+    if constexpr (PASS == kForward) return forward<T, NS>(a, p, s);
+    else if constexpr (PASS == kBackward) return backward<T, NS>(a, p, s);
+    else return step<T, NS>(a, p, s);
+}
+template <typename T, Pass PASS> int by_states(const adn_scan_args& a, const ScanParams& p, int ns, hipStream_t s) {
+    switch (ns) {
+        case 1: return go<T, PASS, 1>(a, p, s);
+        case 2: return go<T, PASS, 2>(a, p, s);
+        case 4: return go<T, PASS, 4>(a, p, s);
+        default: return go<T, PASS, 8>(a, p, s);
+    }
+}
+template <Pass PASS> int dispatch(const adn_scan_args& a, const ScanParams& p, int ns, hipStream_t s) {
+    return a.dtype == ADN_DTYPE_BF16 ? by_states<__bf16, PASS>(a, p, ns, s) : by_states<float, PASS>(a, p, ns, s);
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace adn
+
+using namespace adn;
+using namespace adn::seq;
+
+extern "C" int64_t adn_op_selective_scan_checkpoints(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups) {
+    if (!sizes_ok(batch, steps, channels, states, groups)) return -1;
+    return plan_of(batch, steps, channels, states, groups).ckpt;
+}
+
+extern "C" int64_t adn_op_selective_scan_workspace(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups, int32_t backward) {
+    if (!sizes_ok(batch, steps, channels, states, groups)) return -1;
+    const Plan q = plan_of(batch, steps, channels, states, groups);
+    return backward ? q.part_a + q.part_bc : 0;
+}
+
+extern "C" int adn_op_selective_scan_forward(const adn_scan_args* a, void* hip_stream) {
+    ADN_TRY(check(a, "adn_op_selective_scan_forward", false));
+    if (a->batch == 0) return ADN_OK;
+    ADN_CHECK(a->state_out && a->state_out != a->state, ADN_ERR_INVALID, "adn_op_selective_scan_forward: state_out is null or the state that is read");
+    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups);
+    ADN_CHECK(!a->checkpoints || (ptr_aligned(a->checkpoints, 16) && a->checkpoint_floats >= q.ckpt), ADN_ERR_INVALID,
+              "adn_op_selective_scan_forward: checkpoints smaller than adn_op_selective_scan_checkpoints() floats, or not on 16 bytes");
+    ADN_CHECK((int64_t)a->batch * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_forward: batch too large");
+    return dispatch<kForward>(*a, params(*a, q), q.ns, static_cast<hipStream_t>(hip_stream));
+}
+
+extern "C" int adn_op_selective_scan_backward(const adn_scan_args* a, void* hip_stream) {
+    ADN_TRY(check(a, "adn_op_selective_scan_backward", true));
+    ADN_CHECK(a->dA && a->dD && a->ddelta_bias, ADN_ERR_INVALID, "adn_op_selective_scan_backward: null gradient");
+    const int64_t frames = (int64_t)a->batch * a->steps;
+    ADN_CHECK(frames == 0 || (a->dB && a->dC), ADN_ERR_INVALID, "adn_op_selective_scan_backward: null gradient");
+    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups);
+    ADN_CHECK(q.ckpt == 0 || (a->checkpoints && ptr_aligned(a->checkpoints, 16) && a->checkpoint_floats >= q.ckpt), ADN_ERR_INVALID,
+              "adn_op_selective_scan_backward: needs the checkpoints of the forward pass");
+    ADN_CHECK(q.part_a + q.part_bc == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= q.part_a + q.part_bc), ADN_ERR_INVALID,
+              "adn_op_selective_scan_backward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
+    ADN_CHECK((int64_t)q.nbg * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
+    ScanParams p = params(*a, q);
+    p.part_a = a->workspace;
+    p.part_bc = a->workspace + q.part_a;
+    return dispatch<kBackward>(*a, p, q.ns, static_cast<hipStream_t>(hip_stream));
+}
+
+extern "C" int adn_op_selective_scan_step(const adn_scan_args* a, void* hip_stream) {
+    ADN_TRY(check(a, "adn_op_selective_scan_step", false));
+    if (a->batch == 0) return ADN_OK;
+    ADN_CHECK(a->steps == 1 && !a->lens, ADN_ERR_INVALID, "adn_op_selective_scan_step: one frame, no lengths");
+    ADN_CHECK(a->state_out, ADN_ERR_INVALID, "adn_op_selective_scan_step: null state");
+    const Plan q = plan_of(a->batch, 1, a->channels, a->states, a->groups);
+    return dispatch<kStep>(*a, params(*a, q), q.ns, static_cast<hipStream_t>(hip_stream));
+}
