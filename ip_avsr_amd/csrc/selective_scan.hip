@@ -49,8 +49,8 @@ struct ScanParams {
     int softplus;
 };
 
-// channels of a quad: with NS states per lane, 8 (channel, state) pairs per lane (4 where N <= 4)
-constexpr int channels_per_quad(int ns) { return ns == 8 ? 1 : (ns == 4 ? 2 : 4); }
+// channels of a quad: with NS states per lane, 4 (channel, state) pairs per lane (8 where N > 16)
+constexpr int channels_per_quad(int ns) { return ns == 8 ? 1 : 4 / ns; }
 
 // log(1 + exp(x)), relative accuracy also where it is small: log1p(e) = 2 atanh(e / (2 + e)) of e = exp(-|x|) <= 1, whose odd series
 // in s = e / (2 + e) <= 1/3 is cut where the rest is below 2^-26 of it
