@@ -9,16 +9,18 @@
 // Bound: the vector pipe.  A (t, d, n) costs a multiply, an exp2 (a quarter of the rate), a multiply and two fused multiply-adds
 // forward -- 8 issue slots of a plain instruction -- and about 17 backward, against 8 / N bytes of bfloat16 traffic.
 //
-// Layout: a quad of lanes owns NC channels and splits their states, lane `ng` of it NS of them, so a lane keeps NC NS states and
-// decays in registers and B_t, C_t cost it NS values each (staged through LDS as float32, once for the workgroup).  What belongs to
-// a (frame, channel) and not to a state -- the step size, the gate, all loads and stores -- is done once: the quad covers 4 / NC
-// frames x NC channels, one per lane, and hands dt and dt u round by quad_perm; a sum over the states is a transposing reduction of
-// 4 values over the quad (9 instructions) that leaves each lane the one it owns.  A workgroup is 4 waves of 16 NC channels.
+// Layout: a quad of lanes owns NC channels and splits their states, lane `ng` of it NS of them, so a lane keeps NC NS = 4 states and
+// decays in registers (8 where N > 16) and B_t, C_t cost it NS values each (staged through LDS as float32, once for the workgroup).
+// What belongs to a (frame, channel) and not to a state -- the step size, the gate, all loads and stores -- is done once: the quad
+// covers 4 / NC frames x NC channels, one per lane, and hands dt and dt u round by quad_perm; a sum over the states is a transposing
+// reduction of 4 values over the quad (9 instructions) that leaves each lane the one it owns.  A workgroup is 4 waves of 16 NC
+// channels.  More states per lane would save a tenth of the instructions and cost the registers that the backward pass needs.
 //
-// The backward pass walks segments of 8 frames from the end: from the state the forward pass kept at the segment's start it
-// recomputes a and e of the segment into registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by
-// exchanging halves (permlane swaps, row rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA,
-// dD and the bias' gradient stay in registers over all frames of a workgroup's utterances.  All sums run in a fixed order.
+// Frames go by segments of 8 (4 where N > 16), the loads of the next one in flight; a whole segment has no branch in it.  The backward
+// pass walks them from the end: from the state the forward pass kept at the segment's start it recomputes a and e of the segment into
+// registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by exchanging halves (permlane swaps, row
+// rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
+// over all frames of a workgroup's utterances.  All sums run in a fixed order.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
 
@@ -27,7 +29,6 @@ namespace seq {
 
 namespace {
 
-constexpr int kSeg = 8;               // frames of a segment: what the backward pass recomputes at a time
 constexpr int kMaxStates = 32;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
 
@@ -41,7 +42,7 @@ struct ScanParams {
     float* ckpt;                      // states before every segment: [B][nseg][ctiles][P / 4][64][4], or null
     const float* dlast;               // backward: gradient of state_out, or null
     float* dstate;                    // backward: gradient of state_in, or null
-    float* part_bc;                   // backward: [bpg][B][nseg][G][kSeg][2][4 NS]
+    float* part_bc;                   // backward: [bpg][B][nseg][G][SEG][2][4 NS]
     float* part_a;                    // backward: [nbg][ctiles][64 P + 2 * 16 NC]
     int B, T, D, N, G, Dg;            // Dg = D / G channels per group
     int nseg, tpg, bpg, ctiles;       // segments; waves and workgroups per group; waves of all workgroups along the channels
@@ -49,8 +50,10 @@ struct ScanParams {
     int softplus;
 };
 
-// channels of a quad: with NS states per lane, 4 (channel, state) pairs per lane (8 where N > 16)
+// channels of a quad and frames of a segment: 4 (channel, state) pairs per lane and 8 frames, 8 and 4 where N > 16 -- what a and e of
+// a segment take in registers is the same
 constexpr int channels_per_quad(int ns) { return ns == 8 ? 1 : 4 / ns; }
+constexpr int segment_frames(int ns) { return ns == 8 ? 4 : 8; }
 
 // log(1 + exp(x)), relative accuracy also where it is small: log1p(e) = 2 atanh(e / (2 + e)) of e = exp(-|x|) <= 1, whose odd series
 // in s = e / (2 + e) <= 1/3 is cut where the rest is below 2^-26 of it
@@ -84,13 +87,16 @@ __device__ __forceinline__ float quad_gather(const float (&v)[4], bool b0, bool 
 }
 
 // where a wave and its lanes stand
-template <int NS, int NC> struct Place {
-    static constexpr int TQ = 4 / NC, WC = 16 * NC, P = NC * NS, Q = kSeg / TQ;
-    int lane, wv, ng, cl, g, ctile, c0, cend, oc, otp;
+template <int NS> struct Place {
+    static constexpr int NC = channels_per_quad(NS), SEG = segment_frames(NS), TQ = 4 / NC, WC = 16 * NC, P = NC * NS, Q = SEG / TQ;
+    static constexpr int STAGE = SEG * 8 * NS, SPT = (STAGE + 255) / 256;      // values of B and C in a segment, and per thread
+    int lane, wv, ng, cl, g, ctile, c0, cend, oc, ld, otp;
     bool ocv, b0, b1;
+    int st_s, st_at, st_which;        // the staged value of this thread: frame, place in the row of its group, B or C
+    bool st_on;
     __device__ __forceinline__ Place(const ScanParams& p, int cblk) {
         lane = threadIdx.x & 63;
-        wv = threadIdx.x / 64;
+        wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
         ng = lane & 3;
         cl = lane >> 2;
         g = cblk / p.bpg;
@@ -101,33 +107,44 @@ template <int NS, int NC> struct Place {
         oc = c0 + ng % NC;                          // the channel and, below, the frame of the quad that this lane owns
         otp = ng / NC;
         ocv = oc < cend;
+        ld = min(oc, cend - 1);                     // a lane without a channel loads the last one's and drops it
         b0 = ng & 1;
         b1 = ng >> 1;
+        st_s = (int)threadIdx.x / (8 * NS);
+        st_which = ((int)threadIdx.x / (4 * NS)) & 1;
+        const int n = (int)threadIdx.x % (4 * NS);
+        st_on = (int)threadIdx.x < STAGE && n < p.N;
+        st_at = g * p.N + min(n, p.N - 1);
     }
 };
+static_assert(Place<1>::SPT == 1 && Place<2>::SPT == 1 && Place<4>::SPT == 1 && Place<8>::SPT == 1, "one staged value per thread");
 
-// B and C rows of a segment: value i of kSeg x 2 x 4 NS; 0 behind the length and behind N
-template <typename T, int NS>
-__device__ __forceinline__ float stage_value(const View<const T>& bm, const View<const T>& cm, const ScanParams& p, int b, int g, int t0, int len, int i) {
-    const int s = i / (8 * NS), n = i % (4 * NS), t = t0 + s;
-    if (s >= kSeg || t >= len || t < 0 || n >= p.N) return 0.f;
-    return (float)((i / (4 * NS)) & 1 ? cm : bm).row(b, t)[(int64_t)g * p.N + n];
+// a (B, T, D) tensor as a wave walks one utterance: a uniform pointer to the segment and a 32-bit offset per lane (check() holds the
+// frame stride below 2^28)
+template <typename T> struct Walk {
+    const char* p;
+    uint32_t frame;                    // bytes between frames
+    uint32_t off;
+    __device__ __forceinline__ Walk(const View<T>& v, int b, int frame_of_lane, int c)
+        : p(reinterpret_cast<const char*>(v.p + b * v.sb)), frame((uint32_t)v.st * (uint32_t)sizeof(T)), off((uint32_t)((uint32_t)frame_of_lane * (uint32_t)v.st + (uint32_t)c) * (uint32_t)sizeof(T)) {}
+    // the lane's element, t0 frames on
+    __device__ __forceinline__ T* at(int t0) const { return reinterpret_cast<T*>(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame) + off); }
+};
+
+template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p, int b, int seg, int ctile) {
+    return (((int64_t)b * p.nseg + seg) * p.ctiles + ctile) * 64 * P;
 }
 
-template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p, int b, int seg, int ctile, int lane) {
-    return (((int64_t)b * p.nseg + seg) * p.ctiles + ctile) * 64 * P + lane * 4;
-}
-
-template <typename T, int NS, int NC, bool GATED, bool SAVE>
-__global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
+template <typename T, int NS, bool GATED, bool SAVE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
                                                            View<T> y, ScanParams p) {
-    using L = Place<NS, NC>;
-    constexpr int TQ = L::TQ, P = L::P, Q = L::Q, STAGE = kSeg * 8 * NS, SPT = (STAGE + 255) / 256;
+    using L = Place<NS>;
+    constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, SEG = L::SEG, STAGE = L::STAGE;
     __shared__ __align__(16) float bc[2][STAGE];
     const int cb = p.bpg * p.G;
     const int b = (int)(blockIdx.x / cb);
     const L l(p, (int)(blockIdx.x - (unsigned)b * cb));
-    const int len = valid_steps(p.lens, b, p.T), nv = (len + kSeg - 1) / kSeg;
+    const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
     float A2[NC][NS], h[NC][NS];
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -139,38 +156,50 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View
             h[k][j] = on && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
-    T un[Q], xn[Q], zn[Q];
-    float st[SPT];
+    const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld);
+    const Walk<T> wy(y, b, l.otp, l.ld);
+    const Walk<const T> wb(l.st_which ? cm : bm, b, l.st_s, l.st_at);
+    T un[Q], xn[Q], zn[Q], st;
     auto fetch = [&](int seg) {
-        const int t0 = seg * kSeg;
+        const int t0 = seg * SEG;
+        if (t0 + SEG <= len) {
+            st = *wb.at(t0);
 #pragma unroll
-        for (int m = 0; m < SPT; ++m) st[m] = stage_value<T, NS>(bm, cm, p, b, l.g, t0, len, threadIdx.x + 256 * m);
+            for (int i = 0; i < Q; ++i) {
+                un[i] = *wu.at(t0 + i * TQ);
+                xn[i] = *wx.at(t0 + i * TQ);
+                if (GATED) zn[i] = *wz.at(t0 + i * TQ);
+            }
+        } else {
+            st = t0 + l.st_s < len ? *wb.at(t0) : (T)0.f;
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            const int t = t0 + i * TQ + l.otp;
-            const bool on = l.ocv && t < len;
-            un[i] = on ? u.row(b, t)[l.oc] : (T)0.f;
-            xn[i] = on ? delta.row(b, t)[l.oc] : (T)0.f;
-            if (GATED) zn[i] = on ? z.row(b, t)[l.oc] : (T)0.f;
+            for (int i = 0; i < Q; ++i) {
+                const bool on = t0 + i * TQ + l.otp < len;
+                un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
+                xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
+                if (GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
+            }
         }
     };
     if (nv) fetch(0);
     for (int seg = 0; seg < nv; ++seg) {
         float* buf = bc[seg & 1];
-#pragma unroll
-        for (int m = 0; m < SPT; ++m)
-            if ((int)threadIdx.x + 256 * m < STAGE) buf[threadIdx.x + 256 * m] = st[m];
+        if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
         __syncthreads();            // (the other buffer may still be read by a wave in the segment before)
-        float uc[Q], xc[Q], zc[Q];
+        const int t0 = seg * SEG;
+        const bool full = t0 + SEG <= len;
+        float uc[Q], zc[Q], dt[Q], o[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            uc[i] = (float)un[i];
-            xc[i] = (float)xn[i] + bias;
-            if (GATED) zc[i] = (float)zn[i];
+            uc[i] = l.ocv ? (float)un[i] : 0.f;
+            const float x = l.ocv ? (float)xn[i] + bias : 0.f;
+            if (GATED) zc[i] = l.ocv ? (float)zn[i] : 0.f;
+            dt[i] = p.softplus ? softplusf(x) : x;
+            if (!full) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;      // the state passes a padding frame
         }
         if (seg + 1 < nv) fetch(seg + 1);
         if (SAVE) {
-            float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile, l.lane);
+            float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
             for (int m = 0; m < P / 4; ++m) {
                 float v[4];
@@ -181,9 +210,7 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View
         }
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            const int t = seg * kSeg + i * TQ + l.otp;
-            const float dt = t < len ? (p.softplus ? softplusf(xc[i]) : xc[i]) : 0.f;      // dt = 0: the state passes a padding frame
-            const float dtu = dt * uc[i];
+            const float dtu = dt[i] * uc[i];
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int tp = 0; tp < TQ; ++tp) {
@@ -193,7 +220,7 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View
 #pragma unroll
                 for (int k = 0; k < NC; ++k) {
                     const int q = tp * NC + k;
-                    const float dtk = bcast(dt, q), dtuk = bcast(dtu, q);
+                    const float dtk = bcast(dt[i], q), dtuk = bcast(dtu, q);
 #pragma unroll
                     for (int j = 0; j < NS; ++j) {
                         const float a = __builtin_amdgcn_exp2f(dtk * A2[k][j]);
@@ -202,13 +229,24 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View
                     }
                 }
             }
-            float o = quad_gather(acc, l.b0, l.b1) + Dv * uc[i];
-            if (GATED) o *= zc[i] * sigmoidf(zc[i]);
-            if (l.ocv && t < p.T) y.row(b, t)[l.oc] = (T)(t < len ? o : 0.f);
+            o[i] = quad_gather(acc, l.b0, l.b1) + Dv * uc[i];
+            if (GATED) o[i] *= zc[i] * sigmoidf(zc[i]);
+        }
+        if (l.ocv) {
+            if (full) {
+#pragma unroll
+                for (int i = 0; i < Q; ++i) *wy.at(t0 + i * TQ) = (T)o[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    const int t = t0 + i * TQ + l.otp;
+                    if (t < p.T) *wy.at(t0 + i * TQ) = (T)(t < len ? o[i] : 0.f);
+                }
+            }
         }
     }
-    for (int t = nv * kSeg + l.otp; t < p.T; t += TQ)
-        if (l.ocv) y.row(b, t)[l.oc] = (T)0.f;
+    for (int t = nv * SEG; t < p.T; t += TQ)
+        if (l.ocv && t + l.otp < p.T) *wy.at(t) = (T)0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -218,56 +256,58 @@ __global__ __launch_bounds__(256) void scan_forward_kernel(View<const T> u, View
         }
 }
 
-// sum over the 16 quads of a wave of the 2 NS values of each lane (NS of dB, NS of dC), each sum in one lane per ng: halves are
-// exchanged while there are several values, so a step halves the values and adds one bit of the lane to the place
-template <int NS> __device__ __forceinline__ void reduce_quads(float (&v)[2 * NS], const int lane, float* out) {
+// where reduce_quads leaves a lane's sum in a row of 2 x 4 NS values: behind it (8 NS on, a place nobody reads) where the lane has none
+template <int NS> __device__ __forceinline__ int reduced_at(int lane) {
+    constexpr int V = 2 * NS;
+    int v = (lane >> 5) * (V / 2);
+    bool mine = true;
+    if (V >= 4) v += ((lane >> 4) & 1) * (V / 4);
+    else mine = lane & 16;
+    if (V >= 8) v += ((lane >> 3) & 1) * (V / 8);
+    else mine = mine && (lane & 8);
+    if (V >= 16) v += (lane >> 2) & 1;
+    else mine = mine && (lane & 4);
+    return (v / NS) * 4 * NS + (lane & 3) * NS + v % NS + (mine ? 0 : 8 * NS);
+}
+// sum over the 16 quads of a wave of the 2 NS values of each lane (NS of dB, NS of dC): halves are exchanged while there are several
+// values, so a step halves the values and adds one bit of the lane to the place
+template <int NS> __device__ __forceinline__ float reduce_quads(const float (&v)[2 * NS], const int lane) {
     constexpr int V = 2 * NS;
     float r1[V / 2], r2[(V + 3) / 4];
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) r1[i] = add_swap32(v[i], v[i + V / 2]);
-    int at = (lane >> 5) * (V / 2);
     if constexpr (V >= 4) {
 #pragma unroll
         for (int i = 0; i < V / 4; ++i) r2[i] = add_swap16(r1[i], r1[i + V / 4]);
-        at += ((lane >> 4) & 1) * (V / 4);
     } else {
         r2[0] = add_swap16(r1[0], r1[0]);
     }
     const bool b3 = lane & 8, b2 = lane & 4;
-    bool mine = V >= 4 || (lane & 16);
-    float r;
     if constexpr (V >= 8) {
         float r3[V / 8];
 #pragma unroll
         for (int i = 0; i < V / 8; ++i) r3[i] = (b3 ? r2[i + V / 8] : r2[i]) + dpp<kRowRor8>(b3 ? r2[i] : r2[i + V / 8]);
-        at += b3 ? V / 8 : 0;
-        if constexpr (V >= 16) {
-            const float give = b2 ? r3[0] : r3[1];
-            // lane ^ 4
-            r = (b2 ? r3[1] : r3[0]) + __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, give), 0x101F));
-            at += b2 ? 1 : 0;
-        } else {
-            r = r3[0] + dpp<0x114>(r3[0]);          // row_shr:4: complete in the lanes with bit 2 set
-            mine = mine && b2;
-        }
+        if constexpr (V >= 16)      // the swizzle: lane ^ 4
+            return (b2 ? r3[1] : r3[0]) + __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, b2 ? r3[0] : r3[1]), 0x101F));
+        else
+            return r3[0] + dpp<kRowShr4>(r3[0]);          // complete in the lanes with bit 2 set
     } else {
-        r = r2[0] + dpp<kRowRor8>(r2[0]);
-        r = r + dpp<0x114>(r);
-        mine = mine && b2 && b3;
+        const float r = r2[0] + dpp<kRowRor8>(r2[0]);
+        return r + dpp<kRowShr4>(r);
     }
-    if (mine) out[(at / NS) * 4 * NS + (lane & 3) * NS + at % NS] = r;
 }
 
-template <typename T, int NS, int NC, bool GATED>
-__global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
+template <typename T, int NS, bool GATED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void scan_backward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
                                                                View<const T> dy, View<T> du, View<T> ddelta, View<T> dz, ScanParams p) {
-    using L = Place<NS, NC>;
-    constexpr int TQ = L::TQ, P = L::P, Q = L::Q, WC = L::WC, STAGE = kSeg * 8 * NS, SPT = (STAGE + 255) / 256;
+    using L = Place<NS>;
+    constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, WC = L::WC, SEG = L::SEG, STAGE = L::STAGE;
     __shared__ __align__(16) float bc[2][STAGE];
-    __shared__ float red[2][4][STAGE];
+    __shared__ float red[2][4][SEG][16 * NS];           // per frame 8 NS sums and 8 NS places nobody reads
     const int cb = p.bpg * p.G;
     const int bg = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)bg * cb);
     const L l(p, cblk);
+    const int red_at = reduced_at<NS>(l.lane);
     float A2[NC][NS], dA[NC][NS];
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -280,13 +320,17 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, 
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
     float dD = 0.f, dbias = 0.f;
     int turn = 0;
-    int64_t flush_at = -1;                      // where the sums waiting in red[turn ^ 1] go
-    auto flush = [&](const float (*rd)[STAGE]) {
-        for (int i = threadIdx.x; i < STAGE; i += 256) p.part_bc[flush_at + i] = ((rd[0][i] + rd[1][i]) + rd[2][i]) + rd[3][i];
+    float* flush_at = nullptr;                  // where the sums waiting in red[turn ^ 1] go
+    auto flush = [&](const float (*rd)[SEG][16 * NS]) {
+        const int i = threadIdx.x, s = l.st_s, at = i % (8 * NS);
+        if (i < STAGE) flush_at[i] = ((rd[0][s][at] + rd[1][s][at]) + rd[2][s][at]) + rd[3][s][at];
     };
     const int b_end = min(p.B, (bg + 1) * p.per_bg);
     for (int b = bg * p.per_bg; b < b_end; ++b) {
-        const int len = valid_steps(p.lens, b, p.T), nv = (len + kSeg - 1) / kSeg;
+        const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
+        const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld), wg(dy, b, l.otp, l.ld);
+        const Walk<T> wdu(du, b, l.otp, l.ld), wdx(ddelta, b, l.otp, l.ld), wdz(dz, b, l.otp, l.ld);
+        const Walk<const T> wb(l.st_which ? cm : bm, b, l.st_s, l.st_at);
         float carry[NC][NS];
 #pragma unroll
         for (int k = 0; k < NC; ++k)
@@ -295,54 +339,63 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, 
                 const int c = l.c0 + k, n = l.ng * NS + j;
                 carry[k][j] = p.dlast && c < l.cend && n < p.N ? p.dlast[((int64_t)b * p.D + c) * p.N + n] : 0.f;
             }
-        for (int t = nv * kSeg + l.otp; t < p.T; t += TQ)
-            if (l.ocv) {
-                du.row(b, t)[l.oc] = (T)0.f;
-                ddelta.row(b, t)[l.oc] = (T)0.f;
-                if (GATED) dz.row(b, t)[l.oc] = (T)0.f;
+        for (int t = nv * SEG; t < p.T; t += TQ)
+            if (l.ocv && t + l.otp < p.T) {
+                *wdu.at(t) = (T)0.f;
+                *wdx.at(t) = (T)0.f;
+                if (GATED) *wdz.at(t) = (T)0.f;
             }
-        T un[Q], xn[Q], zn[Q], gn[Q];
-        float st[SPT], hn[P];
+        T un[Q], xn[Q], zn[Q], gn[Q], st;
+        float hn[P];
         auto fetch = [&](int seg) {
-            const int t0 = seg * kSeg;
+            const int t0 = seg * SEG;
+            if (t0 + SEG <= len) {
+                st = *wb.at(t0);
 #pragma unroll
-            for (int m = 0; m < SPT; ++m) st[m] = stage_value<T, NS>(bm, cm, p, b, l.g, t0, len, threadIdx.x + 256 * m);
+                for (int i = 0; i < Q; ++i) {
+                    un[i] = *wu.at(t0 + i * TQ);
+                    xn[i] = *wx.at(t0 + i * TQ);
+                    gn[i] = *wg.at(t0 + i * TQ);
+                    if (GATED) zn[i] = *wz.at(t0 + i * TQ);
+                }
+            } else {
+                st = t0 + l.st_s < len ? *wb.at(t0) : (T)0.f;
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const int t = t0 + i * TQ + l.otp;
-                const bool on = l.ocv && t < len;
-                un[i] = on ? u.row(b, t)[l.oc] : (T)0.f;
-                xn[i] = on ? delta.row(b, t)[l.oc] : (T)0.f;
-                gn[i] = on ? dy.row(b, t)[l.oc] : (T)0.f;
-                if (GATED) zn[i] = on ? z.row(b, t)[l.oc] : (T)0.f;
+                for (int i = 0; i < Q; ++i) {
+                    const bool on = t0 + i * TQ + l.otp < len;
+                    un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
+                    xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
+                    gn[i] = on ? *wg.at(t0 + i * TQ) : (T)0.f;
+                    if (GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
+                }
             }
-            const float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile, l.lane);
+            const float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
             for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(ck + m * 256, hn + m * 4);
         };
         if (nv) fetch(nv - 1);
         for (int seg = nv - 1; seg >= 0; --seg) {
             float* buf = bc[turn];
-#pragma unroll
-            for (int m = 0; m < SPT; ++m)
-                if ((int)threadIdx.x + 256 * m < STAGE) buf[threadIdx.x + 256 * m] = st[m];
+            if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
             __syncthreads();                    // B and C are in; the sums of the segment before are complete
-            if (flush_at >= 0) flush(red[turn ^ 1]);
-            flush_at = ((((int64_t)(cblk - l.g * p.bpg) * p.B + b) * p.nseg + seg) * p.G + l.g) * STAGE;
-            float uc[Q], xc[Q], zc[Q], gc[Q], dt[Q], h[NC][NS];
+            if (flush_at) flush(red[turn ^ 1]);
+            flush_at = p.part_bc + ((((int64_t)(cblk - l.g * p.bpg) * p.B + b) * p.nseg + seg) * p.G + l.g) * STAGE;
+            const int t0 = seg * SEG;
+            const bool full = t0 + SEG <= len;
+            float uc[Q], xc[Q], zc[Q], gc[Q], dt[Q], h[NC][NS], odu[Q], odx[Q], odz[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                const int t = seg * kSeg + i * TQ + l.otp;
-                uc[i] = (float)un[i];
-                xc[i] = (float)xn[i] + bias;
-                gc[i] = (float)gn[i];
-                if (GATED) zc[i] = (float)zn[i];
-                dt[i] = t < len ? (p.softplus ? softplusf(xc[i]) : xc[i]) : 0.f;
+                uc[i] = l.ocv ? (float)un[i] : 0.f;
+                xc[i] = l.ocv ? (float)xn[i] + bias : 0.f;
+                gc[i] = l.ocv ? (float)gn[i] : 0.f;
+                if (GATED) zc[i] = l.ocv ? (float)zn[i] : 0.f;
+                dt[i] = p.softplus ? softplusf(xc[i]) : xc[i];
+                if (!full) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;
             }
 #pragma unroll
             for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
             if (seg > 0) fetch(seg - 1);
-            float a[kSeg][NC][NS], e[kSeg][NC][NS];
+            float a[SEG][NC][NS], e[SEG][NC][NS];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
                 const float dtu = dt[i] * uc[i];
@@ -393,24 +446,26 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, 
                             carry[k][j] = a[s][k][j] * dh;
                         }
                     }
-                    reduce_quads<NS>(sums, l.lane, red[turn][l.wv] + s * 8 * NS);
+                    red[turn][l.wv][s][red_at] = reduce_quads<NS>(sums, l.lane);
                 }
-                const int t = seg * kSeg + i * TQ + l.otp;
                 const float ddtu = quad_gather(s1, l.b0, l.b1), ddec = quad_gather(s2, l.b0, l.b1) * kLn2;
                 float dx = ddec + uc[i] * ddtu;
                 if (p.softplus) dx *= sigmoidf(xc[i]);
-                if (!(t < len)) dx = 0.f;
-                const float duv = dt[i] * ddtu + Dv * dyp;
+                if (!full) dx = t0 + i * TQ + l.otp < len ? dx : 0.f;
+                odu[i] = dt[i] * ddtu + Dv * dyp;
+                odx[i] = dx;
                 dbias += dx;
                 dD += dyp * uc[i];
-                if (l.ocv && t < p.T) {
-                    du.row(b, t)[l.oc] = (T)duv;
-                    ddelta.row(b, t)[l.oc] = (T)dx;
-                }
-                if (GATED) {
-                    const float yp = quad_gather(sy, l.b0, l.b1) + Dv * uc[i];
-                    if (l.ocv && t < p.T) dz.row(b, t)[l.oc] = (T)(gc[i] * yp * sg * (1.f + zc[i] * (1.f - sg)));
-                }
+                if (GATED) odz[i] = gc[i] * (quad_gather(sy, l.b0, l.b1) + Dv * uc[i]) * sg * (1.f + zc[i] * (1.f - sg));
+            }
+            if (l.ocv) {
+#pragma unroll
+                for (int i = 0; i < Q; ++i)
+                    if (full || t0 + i * TQ + l.otp < p.T) {
+                        *wdu.at(t0 + i * TQ) = (T)odu[i];
+                        *wdx.at(t0 + i * TQ) = (T)odx[i];
+                        if (GATED) *wdz.at(t0 + i * TQ) = (T)odz[i];
+                    }
             }
             turn ^= 1;
         }
@@ -424,7 +479,7 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, 
                 }
     }
     __syncthreads();
-    if (flush_at >= 0) flush(red[turn ^ 1]);
+    if (flush_at) flush(red[turn ^ 1]);
     float* out = p.part_a + ((int64_t)bg * p.ctiles + l.ctile) * (64 * P + 2 * WC);
 #pragma unroll
     for (int m = 0; m < P / 4; ++m) {
@@ -443,10 +498,11 @@ __global__ __launch_bounds__(256, 2) void scan_backward_kernel(View<const T> u, 
 
 // the second launch of the backward pass: workgroups [0, nb_bc) add dB and dC over the workgroups of a group, the others dA, dD and
 // the bias' gradient over the groups of utterances
-template <typename T, int NS, int NC>
+template <typename T, int NS>
 __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T* __restrict__ dC, float* __restrict__ dA, float* __restrict__ dD,
                                                           float* __restrict__ dbias, ScanParams p, int nb_bc) {
-    constexpr int P = NC * NS, WC = 16 * NC, STAGE = kSeg * 8 * NS;
+    using L = Place<NS>;
+    constexpr int P = L::P, WC = L::WC, NC = L::NC, SEG = L::SEG, STAGE = L::STAGE;
     if ((int)blockIdx.x < nb_bc) {
         const int64_t gn = (int64_t)p.G * p.N, total = (int64_t)p.B * p.T * gn * 2;
         const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -456,7 +512,7 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
         const int n = (int)(o % p.N), g = (int)(o % gn) / p.N, b = (int)(bt / p.T), t = (int)(bt % p.T);
         float a = 0.f;
         if (t < valid_steps(p.lens, b, p.T)) {
-            const float* src = p.part_bc + (((int64_t)b * p.nseg + t / kSeg) * p.G + g) * STAGE + (t % kSeg) * 8 * NS + which * 4 * NS + n;
+            const float* src = p.part_bc + (((int64_t)b * p.nseg + t / SEG) * p.G + g) * STAGE + (t % SEG) * 8 * NS + which * 4 * NS + n;
             for (int k = 0; k < p.bpg; ++k) a += src[(int64_t)k * p.B * p.nseg * p.G * STAGE];
         }
         (which ? dC : dB)[o] = (T)a;
@@ -528,7 +584,8 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G) {
     q.ns = states_per_lane(N);
     q.nc = channels_per_quad(q.ns);
     const int Dg = D / G, P = q.ns * q.nc, WC = 16 * q.nc;
-    q.nseg = cdiv(T, kSeg);
+    const int seg = segment_frames(q.ns);
+    q.nseg = cdiv(T, seg);
     q.tpg = cdiv(Dg, WC);
     q.bpg = cdiv(q.tpg, 4);
     q.ctiles = q.bpg * G * 4;
@@ -537,7 +594,7 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G) {
     const int64_t want = std::max<int64_t>(1, cdiv(1024, q.bpg * G));
     q.per_bg = (int)std::max<int64_t>(1, B / want);
     q.nbg = cdiv(B, q.per_bg);
-    q.part_bc = (int64_t)q.bpg * B * q.nseg * G * kSeg * 8 * q.ns;
+    q.part_bc = (int64_t)q.bpg * B * q.nseg * G * seg * 8 * q.ns;
     q.part_a = (int64_t)q.nbg * q.ctiles * (64 * P + 2 * WC);
     return q;
 }
@@ -557,6 +614,10 @@ int check(const adn_scan_args* a, const char* who, bool backward) {
     ADN_CHECK(sizes_ok(a->batch, a->steps, a->channels, a->states, a->groups), ADN_ERR_INVALID, std::string(who) + ": batch * channels too large");
     ADN_CHECK(a->A, ADN_ERR_INVALID, std::string(who) + ": null A");
     const int e = a->dtype == ADN_DTYPE_BF16 ? 2 : 4;
+    // 32-bit offsets within a segment: three frames on, and a channel
+    const auto far = [](const adn_seq& t) { return t.data && (t.stride_t < 0 || t.stride_t >= (int64_t)1 << 28); };
+    ADN_CHECK(!far(a->u) && !far(a->delta) && !far(a->b) && !far(a->c) && !far(a->z) && !far(a->y) && !far(a->dy) && !far(a->du) && !far(a->ddelta) && !far(a->dz),
+              ADN_ERR_INVALID, std::string(who) + ": a frame stride outside 0 .. 2^28");
     if ((int64_t)a->batch * a->steps > 0) {
         ADN_CHECK(seq_ok(a->u, e) && seq_ok(a->delta, e) && seq_ok(a->b, e) && seq_ok(a->c, e), ADN_ERR_INVALID, std::string(who) + ": null or misaligned tensor");
         ADN_CHECK(!a->z.data || seq_ok(a->z, e), ADN_ERR_INVALID, std::string(who) + ": misaligned gate");
@@ -578,10 +639,9 @@ ScanParams params(const adn_scan_args& a, const Plan& q) {
 }
 
 template <typename T, int NS> int forward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
-    constexpr int NC = channels_per_quad(NS);
     const dim3 grid((unsigned)((int64_t)p.B * p.bpg * p.G));
 #define ADN_SCAN_GO(GATED, SAVE)                                                                                                                        \
-    hipLaunchKernelGGL((scan_forward_kernel<T, NS, NC, GATED, SAVE>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
+    hipLaunchKernelGGL((scan_forward_kernel<T, NS, GATED, SAVE>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
                        cview<T>(a.z), view<T>(a.y), p)
     if (a.z.data) {
         if (p.ckpt) ADN_SCAN_GO(true, true);
@@ -596,10 +656,9 @@ template <typename T, int NS> int forward(const adn_scan_args& a, const ScanPara
 }
 
 template <typename T, int NS> int backward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
-    constexpr int NC = channels_per_quad(NS);
     const dim3 grid((unsigned)((int64_t)p.nbg * p.bpg * p.G));
 #define ADN_SCAN_GO(GATED)                                                                                                                          \
-    hipLaunchKernelGGL((scan_backward_kernel<T, NS, NC, GATED>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
+    hipLaunchKernelGGL((scan_backward_kernel<T, NS, GATED>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
                        cview<T>(a.z), cview<T>(a.dy), view<T>(a.du), view<T>(a.ddelta), view<T>(a.dz), p)
     if (p.B > 0) {
         if (a.z.data) ADN_SCAN_GO(true);
@@ -610,7 +669,7 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
     const int64_t bc = (int64_t)p.B * p.T * p.G * p.N * 2, rest = (int64_t)p.D * (p.N + 2);
     const int64_t nb_bc = (bc + 255) / 256;
     ADN_CHECK(nb_bc + (rest + 255) / 256 < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
-    hipLaunchKernelGGL((scan_reduce_kernel<T, NS, NC>), dim3((unsigned)(nb_bc + (rest + 255) / 256)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
+    hipLaunchKernelGGL((scan_reduce_kernel<T, NS>), dim3((unsigned)(nb_bc + (rest + 255) / 256)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
                        a.dA, a.dD, a.ddelta_bias, p, (int)nb_bc);
     ADN_HIP_CHECK(hipGetLastError());
     return ADN_OK;

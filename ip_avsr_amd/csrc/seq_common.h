@@ -41,7 +41,7 @@ template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 template <int Q> __device__ __forceinline__ float quad_bcast(float v) { return dpp<Q * 0x55>(v); }
-constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kRowRor4 = 0x124, kRowRor8 = 0x128;
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kRowRor4 = 0x124, kRowRor8 = 0x128, kRowShr4 = 0x114;
 
 // a and b, the upper 32 lanes of a exchanged with the lower 32 of b: their sum holds a's two halves added in the lower lanes, b's in
 // the upper; swap16 does the same for the odd and even rows of 16 lanes
