@@ -43,10 +43,13 @@ struct ScanParams {
     const float* dlast;               // backward: gradient of state_out, or null
     float* dstate;                    // backward: gradient of state_in, or null
     float* part_bc;                   // backward: [bpg][B][nseg][G][SEG][2][4 NS]
-    float* part_a;                    // backward: [nbg][ctiles][64 P + 2 * 16 NC]
+    float* part_a;                    // backward: [nbg][chunks][ctiles][64 P + 2 * 16 NC]
     int B, T, D, N, G, Dg;            // Dg = D / G channels per group
     int nseg, tpg, bpg, ctiles;       // segments; waves and workgroups per group; waves of all workgroups along the channels
     int nbg, per_bg;                  // backward: groups of utterances, utterances per group
+    int chunks, spc;                  // pieces that the time axis is split into, segments of a piece
+    float* local;                     // chunks > 1: what a piece alone leaves, [B][chunks][ctiles][P / 4][64][4] ...
+    float* dsum;                      // ... and its sum of dt, [B][chunks][ctiles][16 NC]
     int softplus;
 };
 
@@ -135,16 +138,40 @@ template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p,
     return (((int64_t)b * p.nseg + seg) * p.ctiles + ctile) * 64 * P;
 }
 
-template <typename T, int NS, bool GATED, bool SAVE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
-                                                           View<T> y, ScanParams p) {
+template <int P> __device__ __forceinline__ int64_t local_at(const ScanParams& p, int b, int chunk, int ctile) {
+    return (((int64_t)b * p.chunks + chunk) * p.ctiles + ctile) * 64 * P;
+}
+// x (a state, or a state's gradient) carried over a piece: x = what the piece alone leaves + exp(A sum dt) x
+template <int NS>
+__device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>& l, int b, int chunk, const float (&A2)[Place<NS>::NC][NS],
+                                           float (&x)[Place<NS>::NC][NS]) {
+    constexpr int P = Place<NS>::P, NC = Place<NS>::NC, WC = Place<NS>::WC;
+    const float* src = p.local + local_at<P>(p, b, chunk, l.ctile) + l.lane * 4;
+    const float* ds = p.dsum + (((int64_t)b * p.chunks + chunk) * p.ctiles + l.ctile) * WC + l.cl * NC;
+    float v[P], d[NC];
+#pragma unroll
+    for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(src + m * 256, v + m * 4);
+    load_vec<float, NC>(ds, d);
+#pragma unroll
+    for (int m = 0; m < P; ++m) x[m / NS][m % NS] = fmaf(__builtin_amdgcn_exp2f(d[m / NS] * A2[m / NS][m % NS]), x[m / NS][m % NS], v[m]);
+}
+
+// first launch over a split time axis: a piece alone.  Forward (BACK = false) the state it leaves, from zeros -- the first piece from the
+// state it is given; backward the gradient of the state before it, nothing coming from behind.  With it the piece's sum of dt.  Pieces
+// that no other one follows (or precedes, backward) are not needed.
+template <typename T, int NS, bool BACK, bool GATED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_local_kernel(View<const T> u, View<const T> delta, View<const T> m,
+                                                                                                View<const T> z, ScanParams p) {
+    // u: dy where BACK;  m: B, or C where BACK
     using L = Place<NS>;
-    constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, SEG = L::SEG, STAGE = L::STAGE;
-    __shared__ __align__(16) float bc[2][STAGE];
+    constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, SEG = L::SEG, WC = L::WC, ROWS = SEG * 4 * NS;
+    __shared__ __align__(16) float bc[2][ROWS];
     const int cb = p.bpg * p.G;
-    const int b = (int)(blockIdx.x / cb);
-    const L l(p, (int)(blockIdx.x - (unsigned)b * cb));
-    const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
+    const int item = (int)(blockIdx.x / cb), b = item / p.chunks, chunk = item - b * p.chunks;
+    const L l(p, (int)(blockIdx.x - (unsigned)item * cb));
+    const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG, last = (nv - 1) / p.spc;
+    if (nv == 0 || (BACK ? chunk > last || chunk == 0 : chunk >= last)) return;      // the whole workgroup
+    const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc);
     float A2[NC][NS], h[NC][NS];
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -153,8 +180,111 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             const int c = l.c0 + k, n = l.ng * NS + j;
             const bool on = c < l.cend && n < p.N;
             A2[k][j] = on ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
-            h[k][j] = on && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+            h[k][j] = !BACK && on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
+    const float bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
+    const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld);
+    const int ms = (int)threadIdx.x / (4 * NS), mn = (int)threadIdx.x % (4 * NS);
+    const bool mon = (int)threadIdx.x < ROWS && mn < p.N;
+    const Walk<const T> wm(m, b, min(ms, SEG - 1), l.g * p.N + min(mn, p.N - 1));
+    T un[Q], xn[Q], zn[Q], st;
+    auto fetch = [&](int seg) {
+        const int t0 = seg * SEG;
+        if (t0 + SEG <= len) {
+            st = *wm.at(t0);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                un[i] = *wu.at(t0 + i * TQ);
+                xn[i] = *wx.at(t0 + i * TQ);
+                if (BACK && GATED) zn[i] = *wz.at(t0 + i * TQ);
+            }
+        } else {
+            st = t0 + min(ms, SEG - 1) < len ? *wm.at(t0) : (T)0.f;
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const bool on = t0 + i * TQ + l.otp < len;
+                un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
+                xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
+                if (BACK && GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
+            }
+        }
+    };
+    float total = 0.f;
+    const int n = s1 - s0;
+    fetch(BACK ? s1 - 1 : s0);
+    for (int k0 = 0; k0 < n; ++k0) {
+        const int seg = BACK ? s1 - 1 - k0 : s0 + k0, t0 = seg * SEG;
+        float* buf = bc[k0 & 1];
+        if ((int)threadIdx.x < ROWS) buf[threadIdx.x] = mon ? (float)st : 0.f;
+        __syncthreads();
+        float in[Q], dt[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const float x = l.ocv ? (float)xn[i] + bias : 0.f;
+            dt[i] = p.softplus ? softplusf(x) : x;
+            if (t0 + SEG > len) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;
+            in[i] = l.ocv ? (float)un[i] : 0.f;
+            if (!BACK) in[i] *= dt[i];
+            else if (GATED) { const float zc = l.ocv ? (float)zn[i] : 0.f; in[i] *= zc * sigmoidf(zc); }
+            total += dt[i];
+        }
+        if (k0 + 1 < n) fetch(BACK ? seg - 1 : seg + 1);
+#pragma unroll
+        for (int ii = 0; ii < Q; ++ii) {
+            const int i = BACK ? Q - 1 - ii : ii;
+#pragma unroll
+            for (int tt = 0; tt < TQ; ++tt) {
+                const int tp = BACK ? TQ - 1 - tt : tt;
+                float mv[NS];
+                load_vec<float, NS>(buf + (i * TQ + tp) * 4 * NS + l.ng * NS, mv);
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const float dtk = bcast(dt[i], tp * NC + k), ink = bcast(in[i], tp * NC + k);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const float a = __builtin_amdgcn_exp2f(dtk * A2[k][j]);
+                        h[k][j] = BACK ? a * fmaf(mv[j], ink, h[k][j]) : fmaf(a, h[k][j], ink * mv[j]);
+                    }
+                }
+            }
+        }
+    }
+    float* out = p.local + local_at<P>(p, b, chunk, l.ctile) + l.lane * 4;
+#pragma unroll
+    for (int q = 0; q < P / 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = h[(q * 4 + j) / NS][(q * 4 + j) % NS];
+        store_vec<float, 4>(out + q * 256, v);
+    }
+    if constexpr (TQ == 4) total += dpp<kQuadXor1>(total);
+    if constexpr (TQ >= 2) total += dpp<kQuadXor2>(total);
+    if (l.otp == 0) p.dsum[(((int64_t)b * p.chunks + chunk) * p.ctiles + l.ctile) * WC + l.cl * NC + l.ng] = total;
+}
+
+template <typename T, int NS, bool GATED, bool SAVE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
+                                                           View<T> y, ScanParams p) {
+    using L = Place<NS>;
+    constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, SEG = L::SEG, STAGE = L::STAGE;
+    __shared__ __align__(16) float bc[2][STAGE];
+    const int cb = p.bpg * p.G;
+    const int item = (int)(blockIdx.x / cb), b = item / p.chunks, chunk = item - b * p.chunks;
+    const L l(p, (int)(blockIdx.x - (unsigned)item * cb));
+    const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
+    const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc);
+    float A2[NC][NS], h[NC][NS];
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int c = l.c0 + k, n = l.ng * NS + j;
+            const bool on = c < l.cend && n < p.N;
+            A2[k][j] = on ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            h[k][j] = on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+        }
+    if (s0 < nv)
+        for (int c = 0; c < chunk; ++c) carry_over<NS>(p, l, b, c, A2, h);
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
     const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld);
     const Walk<T> wy(y, b, l.otp, l.ld);
@@ -181,8 +311,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             }
         }
     };
-    if (nv) fetch(0);
-    for (int seg = 0; seg < nv; ++seg) {
+    if (s0 < s1) fetch(s0);
+    for (int seg = s0; seg < s1; ++seg) {
         float* buf = bc[seg & 1];
         if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
         __syncthreads();            // (the other buffer may still be read by a wave in the segment before)
@@ -197,7 +327,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             dt[i] = p.softplus ? softplusf(x) : x;
             if (!full) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;      // the state passes a padding frame
         }
-        if (seg + 1 < nv) fetch(seg + 1);
+        if (seg + 1 < s1) fetch(seg + 1);
         if (SAVE) {
             float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
@@ -245,8 +375,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             }
         }
     }
-    for (int t = nv * SEG; t < p.T; t += TQ)
-        if (l.ocv && t + l.otp < p.T) *wy.at(t) = (T)0.f;
+    const int end = min(p.T, (s0 + p.spc) * SEG);
+    for (int t = max(nv, s0) * SEG; t < end; t += TQ)
+        if (l.ocv && t + l.otp < end) *wy.at(t) = (T)0.f;
+    if (chunk == max(nv - 1, 0) / p.spc)
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -305,7 +437,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ __align__(16) float bc[2][STAGE];
     __shared__ float red[2][4][SEG][16 * NS];           // per frame 8 NS sums and 8 NS places nobody reads
     const int cb = p.bpg * p.G;
-    const int bg = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)bg * cb);
+    const int item = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)item * cb), bg = item / p.chunks, chunk = item - bg * p.chunks;
     const L l(p, cblk);
     const int red_at = reduced_at<NS>(l.lane);
     float A2[NC][NS], dA[NC][NS];
@@ -339,8 +471,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 const int c = l.c0 + k, n = l.ng * NS + j;
                 carry[k][j] = p.dlast && c < l.cend && n < p.N ? p.dlast[((int64_t)b * p.D + c) * p.N + n] : 0.f;
             }
-        for (int t = nv * SEG; t < p.T; t += TQ)
-            if (l.ocv && t + l.otp < p.T) {
+        const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc), end = min(p.T, (s0 + p.spc) * SEG);
+        if (s0 < nv)
+            for (int c = (nv - 1) / p.spc; c > chunk; --c) carry_over<NS>(p, l, b, c, A2, carry);
+        for (int t = max(nv, s0) * SEG; t < end; t += TQ)
+            if (l.ocv && t + l.otp < end) {
                 *wdu.at(t) = (T)0.f;
                 *wdx.at(t) = (T)0.f;
                 if (GATED) *wdz.at(t) = (T)0.f;
@@ -373,8 +508,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(ck + m * 256, hn + m * 4);
         };
-        if (nv) fetch(nv - 1);
-        for (int seg = nv - 1; seg >= 0; --seg) {
+        if (s0 < s1) fetch(s1 - 1);
+        for (int seg = s1 - 1; seg >= s0; --seg) {
             float* buf = bc[turn];
             if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
             __syncthreads();                    // B and C are in; the sums of the segment before are complete
@@ -394,7 +529,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
 #pragma unroll
             for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
-            if (seg > 0) fetch(seg - 1);
+            if (seg > s0) fetch(seg - 1);
             float a[SEG][NC][NS], e[SEG][NC][NS];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
@@ -469,7 +604,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             turn ^= 1;
         }
-        if (p.dstate)
+        if (p.dstate && chunk == 0)
 #pragma unroll
             for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -480,7 +615,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     __syncthreads();
     if (flush_at) flush(red[turn ^ 1]);
-    float* out = p.part_a + ((int64_t)bg * p.ctiles + l.ctile) * (64 * P + 2 * WC);
+    float* out = p.part_a + ((int64_t)item * p.ctiles + l.ctile) * (64 * P + 2 * WC);
 #pragma unroll
     for (int m = 0; m < P / 4; ++m) {
         float v[4];
@@ -530,7 +665,7 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
     } else
         at = 64 * P + (i - da >= p.D ? WC : 0) + cw;
     float a = 0.f;
-    for (int k = 0; k < p.nbg; ++k) a += p.part_a[row + at + k * stride];
+    for (int k = 0; k < p.nbg * p.chunks; ++k) a += p.part_a[row + at + k * stride];
     if (i < da) dA[i] = a;
     else if (i - da < p.D) dD[c] = a;
     else dbias[c] = a;
@@ -577,9 +712,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u,
 
 int states_per_lane(int n) { return n <= 4 ? 1 : (n <= 8 ? 2 : (n <= 16 ? 4 : 8)); }
 
-struct Plan { int ns, nc, nseg, tpg, bpg, ctiles, nbg, per_bg; int64_t ckpt, part_bc, part_a; };
+constexpr int kMinPiece = 8;           // segments of a piece, at least
 
-Plan plan_of(int64_t B, int64_t T, int D, int N, int G) {
+struct Plan { int ns, nc, nseg, tpg, bpg, ctiles, nbg, per_bg, chunks, spc; int64_t ckpt, part_bc, part_a, local, dsum; };
+
+Plan plan_of(int64_t B, int64_t T, int D, int N, int G, bool bwd) {
     Plan q{};
     q.ns = states_per_lane(N);
     q.nc = channels_per_quad(q.ns);
@@ -594,8 +731,17 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G) {
     const int64_t want = std::max<int64_t>(1, cdiv(1024, q.bpg * G));
     q.per_bg = (int)std::max<int64_t>(1, B / want);
     q.nbg = cdiv(B, q.per_bg);
+    // a time axis in pieces: where the utterances and channels alone leave half of the SIMDs without a wave
+    const int64_t waves = B * q.tpg * G;
+    q.chunks = 1;
+    if (B > 0 && waves <= 512 && q.nseg >= 2 * kMinPiece)
+        q.chunks = (int)std::min<int64_t>(q.nseg / kMinPiece, ((bwd ? 2048 : 4096) + waves - 1) / waves);
+    q.spc = std::max(1, cdiv(q.nseg, q.chunks));
+    q.chunks = std::max(1, cdiv(q.nseg, q.spc));
+    q.local = q.chunks > 1 ? B * q.chunks * q.ctiles * 64 * P : 0;
+    q.dsum = q.chunks > 1 ? B * q.chunks * q.ctiles * WC : 0;
     q.part_bc = (int64_t)q.bpg * B * q.nseg * G * seg * 8 * q.ns;
-    q.part_a = (int64_t)q.nbg * q.ctiles * (64 * P + 2 * WC);
+    q.part_a = (int64_t)q.nbg * q.chunks * q.ctiles * (64 * P + 2 * WC);
     return q;
 }
 
@@ -634,12 +780,15 @@ ScanParams params(const adn_scan_args& a, const Plan& q) {
     p.dlast = a.dlast; p.dstate = a.dstate;
     p.B = a.batch; p.T = a.steps; p.D = a.channels; p.N = a.states; p.G = a.groups; p.Dg = a.channels / a.groups;
     p.nseg = q.nseg; p.tpg = q.tpg; p.bpg = q.bpg; p.ctiles = q.ctiles; p.nbg = q.nbg; p.per_bg = q.per_bg;
+    p.chunks = q.chunks; p.spc = q.spc;
     p.softplus = a.softplus;
     return p;
 }
 
 template <typename T, int NS> int forward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)p.B * p.bpg * p.G));
+    const dim3 grid((unsigned)((int64_t)p.B * p.chunks * p.bpg * p.G));
+    if (p.chunks > 1)
+        hipLaunchKernelGGL((scan_local_kernel<T, NS, false, false>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), View<const T>{}, p);
 #define ADN_SCAN_GO(GATED, SAVE)                                                                                                                        \
     hipLaunchKernelGGL((scan_forward_kernel<T, NS, GATED, SAVE>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
                        cview<T>(a.z), view<T>(a.y), p)
@@ -656,7 +805,11 @@ template <typename T, int NS> int forward(const adn_scan_args& a, const ScanPara
 }
 
 template <typename T, int NS> int backward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)p.nbg * p.bpg * p.G));
+    const dim3 grid((unsigned)((int64_t)p.nbg * p.chunks * p.bpg * p.G));
+    if (p.chunks > 1) {      // (one utterance per group then: the pieces' grid is B x chunks)
+        if (a.z.data) hipLaunchKernelGGL((scan_local_kernel<T, NS, true, true>), grid, dim3(256), 0, s, cview<T>(a.dy), cview<T>(a.delta), cview<T>(a.c), cview<T>(a.z), p);
+        else hipLaunchKernelGGL((scan_local_kernel<T, NS, true, false>), grid, dim3(256), 0, s, cview<T>(a.dy), cview<T>(a.delta), cview<T>(a.c), View<const T>{}, p);
+    }
 #define ADN_SCAN_GO(GATED)                                                                                                                          \
     hipLaunchKernelGGL((scan_backward_kernel<T, NS, GATED>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
                        cview<T>(a.z), cview<T>(a.dy), view<T>(a.du), view<T>(a.ddelta), view<T>(a.dz), p)
@@ -711,24 +864,29 @@ using namespace adn::seq;
 
 extern "C" int64_t adn_op_selective_scan_checkpoints(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups) {
     if (!sizes_ok(batch, steps, channels, states, groups)) return -1;
-    return plan_of(batch, steps, channels, states, groups).ckpt;
+    return plan_of(batch, steps, channels, states, groups, false).ckpt;
 }
 
 extern "C" int64_t adn_op_selective_scan_workspace(int32_t batch, int32_t steps, int32_t channels, int32_t states, int32_t groups, int32_t backward) {
     if (!sizes_ok(batch, steps, channels, states, groups)) return -1;
-    const Plan q = plan_of(batch, steps, channels, states, groups);
-    return backward ? q.part_a + q.part_bc : 0;
+    const Plan q = plan_of(batch, steps, channels, states, groups, backward != 0);
+    return q.local + q.dsum + (backward ? q.part_a + q.part_bc : 0);
 }
 
 extern "C" int adn_op_selective_scan_forward(const adn_scan_args* a, void* hip_stream) {
     ADN_TRY(check(a, "adn_op_selective_scan_forward", false));
     if (a->batch == 0) return ADN_OK;
     ADN_CHECK(a->state_out && a->state_out != a->state, ADN_ERR_INVALID, "adn_op_selective_scan_forward: state_out is null or the state that is read");
-    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups);
+    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups, false);
     ADN_CHECK(!a->checkpoints || (ptr_aligned(a->checkpoints, 16) && a->checkpoint_floats >= q.ckpt), ADN_ERR_INVALID,
               "adn_op_selective_scan_forward: checkpoints smaller than adn_op_selective_scan_checkpoints() floats, or not on 16 bytes");
-    ADN_CHECK((int64_t)a->batch * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_forward: batch too large");
-    return dispatch<kForward>(*a, params(*a, q), q.ns, static_cast<hipStream_t>(hip_stream));
+    ADN_CHECK(q.local == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= q.local + q.dsum), ADN_ERR_INVALID,
+              "adn_op_selective_scan_forward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
+    ADN_CHECK((int64_t)a->batch * q.chunks * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_forward: batch too large");
+    ScanParams p = params(*a, q);
+    p.local = a->workspace;
+    p.dsum = a->workspace + q.local;
+    return dispatch<kForward>(*a, p, q.ns, static_cast<hipStream_t>(hip_stream));
 }
 
 extern "C" int adn_op_selective_scan_backward(const adn_scan_args* a, void* hip_stream) {
@@ -736,15 +894,18 @@ extern "C" int adn_op_selective_scan_backward(const adn_scan_args* a, void* hip_
     ADN_CHECK(a->dA && a->dD && a->ddelta_bias, ADN_ERR_INVALID, "adn_op_selective_scan_backward: null gradient");
     const int64_t frames = (int64_t)a->batch * a->steps;
     ADN_CHECK(frames == 0 || (a->dB && a->dC), ADN_ERR_INVALID, "adn_op_selective_scan_backward: null gradient");
-    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups);
+    const Plan q = plan_of(a->batch, a->steps, a->channels, a->states, a->groups, true);
     ADN_CHECK(q.ckpt == 0 || (a->checkpoints && ptr_aligned(a->checkpoints, 16) && a->checkpoint_floats >= q.ckpt), ADN_ERR_INVALID,
               "adn_op_selective_scan_backward: needs the checkpoints of the forward pass");
-    ADN_CHECK(q.part_a + q.part_bc == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= q.part_a + q.part_bc), ADN_ERR_INVALID,
+    const int64_t need = q.part_a + q.part_bc + q.local + q.dsum;
+    ADN_CHECK(need == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= need), ADN_ERR_INVALID,
               "adn_op_selective_scan_backward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
-    ADN_CHECK((int64_t)q.nbg * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
+    ADN_CHECK((int64_t)q.nbg * q.chunks * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
     ScanParams p = params(*a, q);
-    p.part_a = a->workspace;
-    p.part_bc = a->workspace + q.part_a;
+    p.local = a->workspace;
+    p.dsum = p.local + q.local;
+    p.part_a = p.dsum + q.dsum;
+    p.part_bc = p.part_a + q.part_a;
     return dispatch<kBackward>(*a, p, q.ns, static_cast<hipStream_t>(hip_stream));
 }
 
@@ -753,6 +914,6 @@ extern "C" int adn_op_selective_scan_step(const adn_scan_args* a, void* hip_stre
     if (a->batch == 0) return ADN_OK;
     ADN_CHECK(a->steps == 1 && !a->lens, ADN_ERR_INVALID, "adn_op_selective_scan_step: one frame, no lengths");
     ADN_CHECK(a->state_out, ADN_ERR_INVALID, "adn_op_selective_scan_step: null state");
-    const Plan q = plan_of(a->batch, 1, a->channels, a->states, a->groups);
+    const Plan q = plan_of(a->batch, 1, a->channels, a->states, a->groups, false);
     return dispatch<kStep>(*a, params(*a, q), q.ns, static_cast<hipStream_t>(hip_stream));
 }

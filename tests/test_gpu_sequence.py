@@ -193,7 +193,10 @@ def _scan_inputs(d, shape, N, G, lens, gated, softplus=True, carried=False):
 
 SCAN = [((1, 1, 1), 1, 1, None), ((2, 3, 5), 3, 1, [3, 0]), ((2, 7, 64), 4, 1, None), ((3, 8, 96), 16, 1, [1, 8, 7]), ((2, 9, 130), 16, 2, [2, 9]),
         ((1, 65, 40), 16, 1, None), ((4, 50, 8), 8, 1, [50, 7, 25, 6]), ((2, 40, 252), 16, 3, [33, 12]), ((2, 16, 16), 32, 1, [16, 1]), ((1, 33, 70), 17, 1, None),
-        ((2, 24, 36), 12, 2, None), ((3, 17, 30), 5, 1, [0, 0, 0]), ((5, 12, 600), 8, 1, [1, 2, 12, 11, 9]), ((1, 20, 100), 31, 4, [19]), ((9, 20, 20), 2, 1, None)]
+        ((2, 24, 36), 12, 2, None), ((3, 17, 30), 5, 1, [0, 0, 0]), ((5, 12, 600), 8, 1, [1, 2, 12, 11, 9]), ((1, 20, 100), 31, 4, [19]), ((9, 20, 20), 2, 1, None),
+        # long enough, and few enough rows, for a time axis in pieces
+        ((1, 200, 20), 16, 1, None), ((2, 261, 70), 5, 2, [261, 129]), ((3, 150, 16), 32, 1, [0, 150, 64]), ((2, 300, 40), 4, 1, [300, 1]),
+        ((1, 129, 33), 1, 1, [128])]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
