@@ -32,20 +32,31 @@ struct ConvParams {
 
 // x at frame t of utterance b, channels c .. c + V: the history before 0, zero behind the length
 template <typename T, int V>
-__device__ __forceinline__ void frame(const View<const T>& x, const ConvParams& p, int b, int t, int c, int len, float* out) {
-    if (t >= 0 && t < len) load_vec<T, V>(x.row(b, t) + c, out);
-    else if (t < 0 && p.state) load_vec<T, V>(static_cast<const T*>(p.state) + ((int64_t)b * (p.K - 1) + t + p.K - 1) * p.C + c, out);
-    else
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[j] = 0.f;
+__device__ __forceinline__ vec_t<T, V> frame(const View<const T>& x, const ConvParams& p, int b, int t, int c, int len) {
+    if (t >= 0 && t < len) return load_raw<T, V>(x.row(b, t) + c);
+    if (t < 0 && p.state) return load_raw<T, V>(static_cast<const T*>(p.state) + ((int64_t)b * (p.K - 1) + t + p.K - 1) * p.C + c);
+    return vec_t<T, V>{};
 }
 
-constexpr int kConvChunk = 4;      // frames loaded together
+constexpr int kConvChunk = 4;      // frames loaded together, one chunk ahead of the arithmetic
+
+// frames t .. t + kConvChunk of x; inside the utterance without a branch per frame
+template <typename T, int V>
+__device__ __forceinline__ void frames(const View<const T>& x, const ConvParams& p, int b, int t, int c, int len, vec_t<T, V> (&out)[kConvChunk]) {
+    if (t >= 0 && t + kConvChunk <= len) {
+        const T* row = x.row(b, t) + c;
+#pragma unroll
+        for (int i = 0; i < kConvChunk; ++i) out[i] = load_raw<T, V>(row + i * x.st);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kConvChunk; ++i) out[i] = frame<T, V>(x, p, b, t + i, c, len);
+    }
+}
 
 // workgroup: 64 lanes x V channels, 4 waves = 4 runs
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View<T> y, ConvParams p) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int c = ((int)blockIdx.y * 64 + (int)(threadIdx.x & 63)) * V;
     if (item >= (int64_t)p.B * p.runs || c >= p.C) return;
     const int b = (int)(item / p.runs), ri = (int)(item - (int64_t)b * p.runs);
@@ -57,11 +68,15 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View
     for (int j = 0; j < V; ++j) bias[j] = 0.f;
     if (p.bias) load_vec<float, V>(p.bias + c, bias);
     float win[K - 1 + kConvChunk][V];
+    vec_t<T, V> next[kConvChunk];
+    frames<T, V>(x, p, b, t0, c, len, next);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) frame<T, V>(x, p, b, t0 - (K - 1) + k, c, len, win[k]);
+    for (int k = 0; k < K - 1; ++k) widen<T, V>(frame<T, V>(x, p, b, t0 - (K - 1) + k, c, len), win[k]);
     for (int t = t0; t < t1; t += kConvChunk) {
 #pragma unroll
-        for (int i = 0; i < kConvChunk; ++i) frame<T, V>(x, p, b, t + i, c, len, win[K - 1 + i]);
+        for (int i = 0; i < kConvChunk; ++i) widen<T, V>(next[i], win[K - 1 + i]);
+        if (t + kConvChunk < t1) frames<T, V>(x, p, b, t + kConvChunk, c, len, next);
+        T* row = y.row(b, t) + c;
 #pragma unroll
         for (int i = 0; i < kConvChunk; ++i) {
             float o[V];
@@ -73,7 +88,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View
                 if (p.silu) a *= sigmoidf(a);
                 o[j] = t + i < len ? a : 0.f;
             }
-            if (t + i < t1) store_vec<T, V>(y.row(b, t + i) + c, o);
+            if (t + i < t1) store_vec<T, V>(row + i * y.st, o);
         }
 #pragma unroll
         for (int k = 0; k < K - 1; ++k)
@@ -82,11 +97,8 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View
     }
     if (ri == 0 && p.state_out) {      // the K - 1 frames before frame `len`
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) {
-            float f[V];
-            frame<T, V>(x, p, b, len - (K - 1) + k, c, len, f);
-            store_vec<T, V>(static_cast<T*>(p.state_out) + ((int64_t)b * (K - 1) + k) * p.C + c, f);
-        }
+        for (int k = 0; k < K - 1; ++k)
+            *reinterpret_cast<vec_t<T, V>*>(static_cast<T*>(p.state_out) + ((int64_t)b * (K - 1) + k) * p.C + c) = frame<T, V>(x, p, b, len - (K - 1) + k, c, len);
     }
 }
 
@@ -94,7 +106,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, View<const T> dy, View<T> dx, ConvParams p) {
     __shared__ float comb[4][(K + 1) * 64 * V];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x / 64;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int c = ((int)blockIdx.y * 64 + lane) * V;
     float dw[K + 1][V];
 #pragma unroll
@@ -112,29 +124,44 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
         for (int64_t item = (int64_t)blockIdx.x * 4 + wv; item < items; item += (int64_t)p.parts * 4) {
             const int b = (int)(item / p.runs), ri = (int)(item - (int64_t)b * p.runs);
             const int t0 = ri * p.run, t1 = min(p.T, t0 + p.run), len = valid_steps(p.lens, b, p.T);
+            const auto gradients = [&](int t, vec_t<T, V> (&out)[kConvChunk]) {
+                if (t + kConvChunk <= len) {
+                    const T* row = dy.row(b, t) + c;
+#pragma unroll
+                    for (int i = 0; i < kConvChunk; ++i) out[i] = load_raw<T, V>(row + i * dy.st);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kConvChunk; ++i) out[i] = t + i < len ? load_raw<T, V>(dy.row(b, t + i) + c) : vec_t<T, V>{};
+                }
+            };
             // dx of frames t0 .. t1 needs dpre of t0 .. t1 + K - 1; the history's gradient is dx at -(K-1) .. 0, the first run's
             float xw[K - 1 + kConvChunk][V], pw[K - 1 + kConvChunk][V];
+            vec_t<T, V> xn[kConvChunk], gn[kConvChunk];
+            frames<T, V>(x, p, b, t0, c, len, xn);
+            gradients(t0, gn);
 #pragma unroll
             for (int k = 0; k < K - 1; ++k) {
-                frame<T, V>(x, p, b, t0 - (K - 1) + k, c, len, xw[k]);
+                widen<T, V>(frame<T, V>(x, p, b, t0 - (K - 1) + k, c, len), xw[k]);
 #pragma unroll
                 for (int j = 0; j < V; ++j) pw[k][j] = 0.f;
             }
             // step t brings dpre[t] and finishes dx[t - (K - 1)].  Before a run's start the window holds zeros for the dpre of earlier
-            // frames: dx[t - (K - 1)] for t < t0 + K - 1 is then incomplete and belongs to the run before (or to the history)
-            for (int t = t0; t < t1 + K - 1; t += kConvChunk) {
+            // frames: dx[t - (K - 1)] for t < t0 + K - 1 is then incomplete and belongs to the run before (or to the history).  Behind
+            // the run's last frame, and behind the length, dpre adds to dx only, and behind the length it is zero
+            const int stop = t1 + K - 1;
+            for (int t = t0; t < stop; t += kConvChunk) {
                 float g[kConvChunk][V];
 #pragma unroll
                 for (int i = 0; i < kConvChunk; ++i) {
-                    frame<T, V>(x, p, b, t + i, c, len, xw[K - 1 + i]);
-                    if (t + i < len) load_vec<T, V>(dy.row(b, t + i) + c, g[i]);
-                    else
-#pragma unroll
-                        for (int j = 0; j < V; ++j) g[i][j] = 0.f;
+                    widen<T, V>(xn[i], xw[K - 1 + i]);
+                    widen<T, V>(gn[i], g[i]);
+                }
+                if (t + kConvChunk < stop) {
+                    frames<T, V>(x, p, b, t + kConvChunk, c, len, xn);
+                    gradients(t + kConvChunk, gn);
                 }
 #pragma unroll
                 for (int i = 0; i < kConvChunk; ++i) {
-                    const bool own = t + i < t1;           // the dpre behind the run's end adds to dx only
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
@@ -147,14 +174,10 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
                             d = t + i < len ? d * (sg * (1.f + a * (1.f - sg))) : 0.f;
                         }
                         pw[K - 1 + i][j] = d;
-                        const float dd = own ? d : 0.f;
-                        dw[K][j] += dd;
+                        float q = 0.f;
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][j] += dd * xw[i + k][j];
-                        float a = 0.f;
-#pragma unroll
-                        for (int k = 0; k < K; ++k) a += w[k][j] * pw[i + K - 1 - k][j];
-                        o[j] = a;
+                        for (int k = 0; k < K; ++k) q += w[k][j] * pw[i + K - 1 - k][j];
+                        o[j] = q;
                     }
                     const int s = t + i - (K - 1);
                     if (s >= t0 && s < t1) {
@@ -164,6 +187,15 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
                         store_vec<T, V>(dx.row(b, s) + c, o);
                     } else if (s < 0 && p.dstate)
                         store_vec<T, V>(static_cast<T*>(p.dstate) + ((int64_t)b * (K - 1) + s + K - 1) * p.C + c, o);
+                    if (t + i < t1) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            const float d = pw[K - 1 + i][j];
+                            dw[K][j] += d;
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dw[k][j] += d * xw[i + k][j];
+                        }
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < K - 1; ++k)
@@ -225,17 +257,18 @@ int check(const adn_conv_args* a, const char* who) {
     return ADN_OK;
 }
 
-// time steps of a run: long ones read fewer frames twice, short ones fill the chip (one workgroup holds four runs of 64 V channels)
-int run_length(int64_t B, int64_t T, int cblocks, int longest) {
-    int run = longest;
-    while (run > 8 && B * ((T + run - 1) / run) * cblocks < 4 * 2048) run /= 2;
-    return run;
+// time steps of a run, of 64 V channels: as long as 2048 waves (two per SIMD) are left -- short runs read more frames twice -- and of
+// about equal length in an utterance
+int run_length(int64_t B, int64_t T, int cblocks) {
+    int64_t runs = (T + 63) / 64;
+    while (B * runs * cblocks < 2048 && (T + runs - 1) / runs > 8) runs *= 2;
+    return (int)std::max<int64_t>((T + runs - 1) / runs, std::min<int64_t>(T, 8));
 }
 constexpr int kConvBwdV = 4;
 // backward: workgroups along the runs; two waves per SIMD over the whole launch
 int conv_parts(int64_t B, int64_t T, int C, int v, int* run) {
     const int cblocks = cdiv(C, 64 * v);
-    *run = run_length(B, T, cblocks, 64);
+    *run = run_length(B, T, cblocks);
     const int64_t items = B * ((T + *run - 1) / *run);
     return (int)std::max<int64_t>(1, std::min<int64_t>((items + 3) / 4, cdiv(1024, cblocks)));
 }
@@ -310,7 +343,7 @@ extern "C" int adn_op_causal_conv_forward(const adn_conv_args* a, void* hip_stre
     const int v = a->dtype == ADN_DTYPE_BF16 ? 8 : 4;
     const bool al = a->channels % v == 0 && seq_aligned(a->x, e, 16) && seq_aligned(a->y, e, 16) && ptr_aligned(a->weight, 16) && ptr_aligned(a->bias, 16) &&
                     ptr_aligned(a->state, 16) && ptr_aligned(a->state_out, 16);
-    p.run = run_length(p.B, std::max(p.T, 1), cdiv(p.C, 64 * (al ? v : 1)), 64);
+    p.run = run_length(p.B, std::max(p.T, 1), cdiv(p.C, 64 * (al ? v : 1)));
     p.runs = std::max(1, cdiv(p.T, p.run));      // (no frames: the history is still handed on)
     ADN_CHECK((int64_t)p.B * p.runs < (int64_t)1 << 32, ADN_ERR_INVALID, "adn_op_causal_conv_forward: batch too large");
     if (a->dtype == ADN_DTYPE_BF16) return al ? launch<__bf16, 8, kForward>(*a, p, s) : launch<__bf16, 1, kForward>(*a, p, s);

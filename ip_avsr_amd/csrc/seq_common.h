@@ -18,6 +18,11 @@ template <typename T> static inline View<const T> cview(const adn_seq& s) { retu
 
 template <typename T, int V> using vec_t = T __attribute__((ext_vector_type(V)));
 
+template <typename T, int V> __device__ __forceinline__ vec_t<T, V> load_raw(const T* __restrict__ p) { return *reinterpret_cast<const vec_t<T, V>*>(p); }
+template <typename T, int V> __device__ __forceinline__ void widen(const vec_t<T, V>& v, float* out) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+}
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* __restrict__ p, float* out) {
     const vec_t<T, V> v = *reinterpret_cast<const vec_t<T, V>*>(p);
 #pragma unroll
