@@ -23,6 +23,8 @@ from .._lib import ConvArgs, NormArgs, ScanArgs
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 _ACTIVATION = {None: 0, "linear": 0, "silu": 1}
 _NO_SEQ = (None, 0, 0)
+# the current stream's handle without the Stream object around it (2.7 us of the 12 of a small call), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _fail(what):
@@ -31,25 +33,22 @@ def _fail(what):
 
 def _activation(name, t, shape, like=None):
     """Checks an activation and returns its (pointer, utterance stride, frame stride)."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        _fail("%s must be a CUDA tensor" % name)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        _fail("%s must be %s on %s, got %s on %s" % (name, like.dtype, like.device, t.dtype, t.device))
-    if t.shape != shape:
-        _fail("%s must have the shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if like is not None:
+        if not isinstance(t, torch.Tensor) or t.dtype is not like.dtype or t.get_device() != like.get_device():
+            _fail("%s must be a %s tensor on %s" % (name, like.dtype, like.device))
+        if t.shape != shape:
+            _fail("%s must have the shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     st = t.stride()
     if st[-1] != 1 and shape[-1] != 1:
         _fail("the channels of %s must be dense" % name)
-    if len(shape) == 3:
-        return t.data_ptr(), st[0], st[1]
-    return t.data_ptr(), st[0], 0
+    return t.data_ptr(), st[0], st[1] if len(st) == 3 else 0
 
 
 def _param(name, t, shape, like, dtype=torch.float32):
     """Checks a dense float32 (or ``dtype``) tensor and returns its pointer; None stays None."""
     if t is None:
         return None
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == like.device and t.shape == shape and t.is_contiguous()):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == like.get_device() and t.shape == shape and t.is_contiguous()):
         _fail("%s must be a dense %s tensor of shape %s on %s" % (name, dtype, tuple(shape), like.device))
     return t.data_ptr()
 
@@ -63,21 +62,24 @@ def _first(name, x, dims):
         _fail("%s must have %s dimensions, got %d" % (name, " or ".join(str(d) for d in dims), x.dim()))
 
 
-def _call(fn, args, device):
-    """Runs an entry point on the current stream of ``device`` (the library launches on the current device)."""
-    if device.index == torch.cuda.current_device():
-        status = fn(args, torch.cuda.current_stream().cuda_stream)
+def _call(fn, args, x):
+    """Runs an entry point on the current stream of x's device (the library launches on the current device)."""
+    index = x.get_device()
+    if index == torch.cuda.current_device():
+        status = fn(args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            status = fn(args, _raw_stream(index))
     if status != _lib.ADN_OK:
         _lib.check(status)
 
 
-def _floats(n, device):
+def _floats(n, x):
+    """(n floats or None, their address)"""
     if n < 0:
         _fail("sizes out of range")
-    return torch.empty(n, dtype=torch.float32, device=device) if n else None
+    ws = x.new_empty(n, dtype=torch.float32) if n else None
+    return ws, (ws.data_ptr() if n else None)
 
 
 # ----------------------------------------------------------------------------------------------------------------- layer norm
@@ -90,12 +92,11 @@ def layer_norm_forward(x, gamma=None, beta=None, lens=None, eps=1e-5):
         y, mean, inv = layer_norm_forward(x[None], gamma, beta, lens, eps)
         return y[0], mean[0], inv[0]
     B, T, D = x.shape
-    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, B, T), dtype=torch.float32, device=x.device)
-    mean, inv = stats[0], stats[1]
+    y = x.new_empty((B, T, D))
+    mean, inv = x.new_empty((B, T), dtype=torch.float32), x.new_empty((B, T), dtype=torch.float32)
     args = NormArgs(_DTYPE[x.dtype], B, T, D, eps, 0, _param("lens", lens, (B,), x, torch.int32), *_activation("x", x, x.shape),
                     y.data_ptr(), T * D, D, _param("gamma", gamma, (D,), x), _param("beta", beta, (D,), x), mean.data_ptr(), inv.data_ptr())
-    _call(_lib.load().adn_op_layer_norm_forward, args, x.device)
+    _call(_lib.load().adn_op_layer_norm_forward, args, x)
     return y, mean, inv
 
 
@@ -108,16 +109,15 @@ def layer_norm_backward(dy, x, gamma, mean, inv_std, lens=None):
         return dx[0], dgamma, dbeta
     B, T, D = x.shape
     lib = _lib.load()
-    dx = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-    grads = torch.empty((2, D), dtype=torch.float32, device=x.device)
+    dx = x.new_empty((B, T, D))
+    dgamma, dbeta = x.new_empty(D, dtype=torch.float32), x.new_empty(D, dtype=torch.float32)
     n = lib.adn_op_layer_norm_workspace(B, T, D)
-    ws = _floats(n, x.device)
+    ws, at = _floats(n, x)
     args = NormArgs(_DTYPE[x.dtype], B, T, D, 0.0, 0, _param("lens", lens, (B,), x, torch.int32), *_activation("x", x, x.shape), *_NO_SEQ,
                     _param("gamma", gamma, (D,), x), None, _param("mean", mean, (B, T), x), _param("inv_std", inv_std, (B, T), x),
-                    *_activation("dy", dy, x.shape, x), dx.data_ptr(), T * D, D, grads[0].data_ptr(), grads[1].data_ptr(),
-                    ws.data_ptr() if n else None, n)
-    _call(lib.adn_op_layer_norm_backward, args, x.device)
-    return dx, grads[0], grads[1]
+                    *_activation("dy", dy, x.shape, x), dx.data_ptr(), T * D, D, dgamma.data_ptr(), dbeta.data_ptr(), at, n)
+    _call(lib.adn_op_layer_norm_backward, args, x)
+    return dx, dgamma, dbeta
 
 
 # ---------------------------------------------------------------------------------------------------- short causal convolution
@@ -138,11 +138,10 @@ def causal_conv_forward(x, weight, bias=None, state=None, lens=None, activation=
     _first("x", x, (3,))
     B, T, D = x.shape
     K, act, w, b = _conv_args(x, weight, bias, lens, activation)
-    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-    out = torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device)
+    y, out = x.new_empty((B, T, D)), x.new_empty((B, K - 1, D))
     args = ConvArgs(_DTYPE[x.dtype], B, T, D, K, act, _param("lens", lens, (B,), x, torch.int32), *_activation("x", x, x.shape),
                     y.data_ptr(), T * D, D, w, b, _param("state", state, (B, K - 1, D), x, x.dtype), out.data_ptr())
-    _call(_lib.load().adn_op_causal_conv_forward, args, x.device)
+    _call(_lib.load().adn_op_causal_conv_forward, args, x)
     return y, out
 
 
@@ -153,16 +152,16 @@ def causal_conv_backward(dy, x, weight, bias=None, state=None, lens=None, activa
     B, T, D = x.shape
     K, act, w, b = _conv_args(x, weight, bias, lens, activation)
     lib = _lib.load()
-    dx = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-    grads = torch.empty((K + 1, D), dtype=torch.float32, device=x.device)
-    dstate = None if state is None else torch.empty((B, K - 1, D), dtype=x.dtype, device=x.device)
+    dx = x.new_empty((B, T, D))
+    dw, db = x.new_empty((K, D), dtype=torch.float32), x.new_empty(D, dtype=torch.float32)
+    dstate = None if state is None else x.new_empty((B, K - 1, D))
     n = lib.adn_op_causal_conv_workspace(B, T, D, K)
-    ws = _floats(n, x.device)
+    ws, at = _floats(n, x)
     args = ConvArgs(_DTYPE[x.dtype], B, T, D, K, act, _param("lens", lens, (B,), x, torch.int32), *_activation("x", x, x.shape), *_NO_SEQ, w, b,
                     _param("state", state, (B, K - 1, D), x, x.dtype), None, *_activation("dy", dy, x.shape, x), dx.data_ptr(), T * D, D,
-                    grads.data_ptr(), grads[K].data_ptr(), None if dstate is None else dstate.data_ptr(), ws.data_ptr() if n else None, n)
-    _call(lib.adn_op_causal_conv_backward, args, x.device)
-    return dx, grads[:K], grads[K], dstate
+                    dw.data_ptr(), db.data_ptr(), None if dstate is None else dstate.data_ptr(), at, n)
+    _call(lib.adn_op_causal_conv_backward, args, x)
+    return dx, dw, db, dstate
 
 
 def causal_conv_step(x, state, weight, bias=None, activation="silu"):
@@ -170,35 +169,36 @@ def causal_conv_step(x, state, weight, bias=None, activation="silu"):
     _first("x", x, (2,))
     B, D = x.shape
     K, act, w, b = _conv_args(x, weight, bias, None, activation)
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    y = x.new_empty((B, D))
     if state is None:
         _fail("a step needs the state it moves on")
     args = ConvArgs(_DTYPE[x.dtype], B, 1, D, K, act, None, *_activation("x", x, x.shape), y.data_ptr(), D, D, w, b,
                     None, _param("state", state, (B, K - 1, D), x, x.dtype))
-    _call(_lib.load().adn_op_causal_conv_step, args, x.device)
+    _call(_lib.load().adn_op_causal_conv_step, args, x)
     return y
 
 
 # ------------------------------------------------------------------------------------------------------ selective state-space scan
 def _scan_rows(name, m, lead, D, N, u):
     """Checks B or C, (..., states) or (..., groups, states) with dense groups and states; returns (groups, pointer and strides)."""
-    if not (isinstance(m, torch.Tensor) and m.is_cuda):
-        _fail("%s must be a CUDA tensor" % name)
-    if m.dim() == len(lead) + 1:
+    if not isinstance(m, torch.Tensor) or m.dtype is not u.dtype or m.get_device() != u.get_device():
+        _fail("%s must be a %s tensor on %s" % (name, u.dtype, u.device))
+    shape, st, k = m.shape, m.stride(), len(lead)
+    if len(shape) == k + 1:
         G = 1
-    elif m.dim() == len(lead) + 2:
-        G = m.shape[-2]
-        if G > 1 and m.stride(-2) != N:
+    elif len(shape) == k + 2:
+        G = shape[-2]
+        if G > 1 and st[-2] != N:
             _fail("the groups of %s must be dense" % name)
         if G < 1 or D % G:
             _fail("%d channels cannot be shared out over the %d groups of %s" % (D, G, name))
     else:
         _fail("%s must be (..., states) or (..., groups, states)" % name)
-    if m.dtype != u.dtype or m.device != u.device or m.shape[:len(lead)] != lead or m.shape[-1] != N:
-        _fail("%s must be %s of %s frames x %d states on %s" % (name, u.dtype, tuple(lead), N, u.device))
-    if m.stride(-1) != 1 and N != 1:
+    if shape[:k] != lead or shape[-1] != N:
+        _fail("%s must hold %d states for each of %s frames, got %s" % (name, N, tuple(lead), tuple(shape)))
+    if st[-1] != 1 and N != 1:
         _fail("the states of %s must be dense" % name)
-    return G, (m.data_ptr(), m.stride(0), m.stride(1) if len(lead) == 2 else 0)
+    return G, (m.data_ptr(), st[0], st[1] if k == 2 else 0)
 
 
 def _scan_head(u, delta, A, Bm, Cm, D, z, delta_bias, lens, softplus, steps):
@@ -211,8 +211,6 @@ def _scan_head(u, delta, A, Bm, Cm, D, z, delta_bias, lens, softplus, steps):
     G2, c = _scan_rows("Cm", Cm, lead, ch, N, u)
     if G != G2:
         _fail("Bm has %d groups, Cm %d" % (G, G2))
-    if N == 1 and (Bm.dim() == len(lead) + 2) and G > 1 and (Bm.stride(-2) != 1 or Cm.stride(-2) != 1):
-        _fail("the groups of Bm and Cm must be dense")
     sizes = (_DTYPE[u.dtype], u.shape[0], steps, ch, N, G, 1 if softplus else 0, 0, _param("lens", lens, (u.shape[0],), u, torch.int32))
     seqs = _activation("u", u, u.shape) + _activation("delta", delta, u.shape, u) + b + c + (_NO_SEQ if z is None else _activation("z", z, u.shape, u))
     return sizes, seqs, (_param("A", A, (ch, N), u), _param("D", D, (ch,), u), _param("delta_bias", delta_bias, (ch,), u))
@@ -232,19 +230,16 @@ def selective_scan_forward(u, delta, A, Bm, Cm, D=None, z=None, delta_bias=None,
     B, T, ch = u.shape
     N, G = sizes[4], sizes[5]
     lib = _lib.load()
-    y = torch.empty((B, T, ch), dtype=u.dtype, device=u.device)
-    out = torch.empty((B, ch, N), dtype=torch.float32, device=u.device)
+    y, out = u.new_empty((B, T, ch)), u.new_empty((B, ch, N), dtype=torch.float32)
     saved, n = None, 0
     if save:
         n = lib.adn_op_selective_scan_checkpoints(B, T, ch, N, G)
-        saved = _floats(n, u.device)
-        if saved is None:
-            saved = torch.empty(0, dtype=torch.float32, device=u.device)
+        saved = u.new_empty(max(n, 0), dtype=torch.float32)
     m = lib.adn_op_selective_scan_workspace(B, T, ch, N, G, 0)
-    ws = _floats(m, u.device)
+    ws, at = _floats(m, u)
     args = ScanArgs(*sizes, *seqs, y.data_ptr(), T * ch, ch, *params, _param("state", state, (B, ch, N), u), out.data_ptr(),
-                    saved.data_ptr() if n else None, n, ws.data_ptr() if m else None, m)
-    _call(lib.adn_op_selective_scan_forward, args, u.device)
+                    saved.data_ptr() if n else None, n, at, m)
+    _call(lib.adn_op_selective_scan_forward, args, u)
     return y, out, saved
 
 
@@ -257,27 +252,23 @@ def selective_scan_backward(dy, u, delta, A, Bm, Cm, saved, D=None, z=None, delt
     B, T, ch = u.shape
     N, G = sizes[4], sizes[5]
     lib = _lib.load()
-    dev = u.device
     n = lib.adn_op_selective_scan_checkpoints(B, T, ch, N, G)
-    _param("saved", saved, (n,), u)
     if saved is None:
         _fail("the backward pass needs what the forward pass saved (save=True)")
+    _param("saved", saved, (n,), u)
     _param("state", state, (B, ch, N), u)
-    du = torch.empty((B, T, ch), dtype=u.dtype, device=dev)
-    ddelta = torch.empty((B, T, ch), dtype=u.dtype, device=dev)
-    dz = None if z is None else torch.empty((B, T, ch), dtype=u.dtype, device=dev)
-    dbc = torch.empty((2,) + tuple(Bm.shape), dtype=u.dtype, device=dev)
-    dA = torch.empty((ch, N), dtype=torch.float32, device=dev)
-    rows = torch.empty((2, ch), dtype=torch.float32, device=dev)
-    dstate = None if state is None else torch.empty((B, ch, N), dtype=torch.float32, device=dev)
+    du, ddelta, dz = u.new_empty((B, T, ch)), u.new_empty((B, T, ch)), None if z is None else u.new_empty((B, T, ch))
+    dB, dC = u.new_empty(Bm.shape), u.new_empty(Cm.shape)
+    dA, dD, dbias = u.new_empty((ch, N), dtype=torch.float32), u.new_empty(ch, dtype=torch.float32), u.new_empty(ch, dtype=torch.float32)
+    dstate = None if state is None else u.new_empty((B, ch, N), dtype=torch.float32)
     m = lib.adn_op_selective_scan_workspace(B, T, ch, N, G, 1)
-    ws = _floats(m, dev)
-    args = ScanArgs(*sizes, *seqs, *_NO_SEQ, *params, None, None, saved.data_ptr() if n else None, n, ws.data_ptr() if m else None, m,
+    ws, at = _floats(m, u)
+    args = ScanArgs(*sizes, *seqs, *_NO_SEQ, *params, None, None, saved.data_ptr() if n else None, n, at, m,
                     *_activation("dy", dy, u.shape, u), du.data_ptr(), T * ch, ch, ddelta.data_ptr(), T * ch, ch,
-                    *(_NO_SEQ if z is None else (dz.data_ptr(), T * ch, ch)), _param("dlast", dlast, (B, ch, N), u), dbc[0].data_ptr(),
-                    dbc[1].data_ptr(), dA.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), None if dstate is None else dstate.data_ptr())
-    _call(lib.adn_op_selective_scan_backward, args, dev)
-    return {"du": du, "ddelta": ddelta, "dz": dz, "dB": dbc[0], "dC": dbc[1], "dA": dA, "dD": rows[0], "ddelta_bias": rows[1], "dstate": dstate}
+                    *(_NO_SEQ if z is None else (dz.data_ptr(), T * ch, ch)), _param("dlast", dlast, (B, ch, N), u), dB.data_ptr(), dC.data_ptr(),
+                    dA.data_ptr(), dD.data_ptr(), dbias.data_ptr(), None if dstate is None else dstate.data_ptr())
+    _call(lib.adn_op_selective_scan_backward, args, u)
+    return {"du": du, "ddelta": ddelta, "dz": dz, "dB": dB, "dC": dC, "dA": dA, "dD": dD, "ddelta_bias": dbias, "dstate": dstate}
 
 
 def selective_scan_step(u, delta, A, Bm, Cm, state, D=None, z=None, delta_bias=None, softplus=True):
@@ -288,7 +279,7 @@ def selective_scan_step(u, delta, A, Bm, Cm, state, D=None, z=None, delta_bias=N
     B, ch = u.shape
     if state is None:
         _fail("a step needs the state it moves on")
-    y = torch.empty((B, ch), dtype=u.dtype, device=u.device)
+    y = u.new_empty((B, ch))
     args = ScanArgs(*sizes, *seqs, y.data_ptr(), ch, ch, *params, None, _param("state", state, (B, ch, sizes[4]), u))
-    _call(_lib.load().adn_op_selective_scan_step, args, u.device)
+    _call(_lib.load().adn_op_selective_scan_step, args, u)
     return y
