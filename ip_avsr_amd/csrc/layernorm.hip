@@ -4,9 +4,9 @@
 //   g = dy gamma:  dx = inv (g - E[g] - xhat E[g xhat]),  dgamma = sum over rows of dy xhat,  dbeta = sum of dy
 //
 // Bound: HBM, one read of x (and dy) and one write of y (dx).  A row lives in registers from its load to its store -- the mean first,
-// then the centred second moment, so nothing cancels -- spread over 64, 256 or 1024 threads (the fewest that keep it to 16 values
-// per thread: more registers per thread cost the waves that hide the loads).  The workgroups are persistent: gamma and beta stay in
-// registers over all their rows, and the backward pass adds dgamma / dbeta there too, leaves one partial row per workgroup, and a
+// then the centred second moment, so nothing cancels -- spread over 64, 256, 512 or 1024 threads (the fewest that keep it to 16 values
+// per thread, forward on one wave 32: more registers per thread cost the waves that hide the loads).  The workgroups are persistent:
+// gamma and beta stay in registers over all their rows, the next row's loads are in flight during a row's sums, and the backward pass adds dgamma / dbeta there too, leaves one partial row per workgroup, and a
 // second launch adds those in a fixed order -- the same bits on every run.
 // Frames at and behind lens[b] are padding: not read, zero in every result, absent from the sums.
 #include "seq_common.h"
@@ -48,26 +48,67 @@ template <int TPR, int K> __device__ __forceinline__ void row_sums(float (&v)[K]
     }
 }
 
+// the rows that a wave, or a workgroup, walks
+struct RowCursor {
+    int r, b, t, step;
+    bool valid;
+    __device__ __forceinline__ RowCursor(const NormParams& p, int first, int by) : r(first), step(by) { place(p); }
+    __device__ __forceinline__ void place(const NormParams& p) {
+        if (r < p.rows) {
+            b = r / p.T;
+            t = r - b * p.T;
+            valid = t < valid_steps(p.lens, b, p.T);
+        } else
+            valid = false;
+    }
+    __device__ __forceinline__ void advance(const NormParams& p) { r += step; place(p); }
+};
+template <int TPR> __device__ __forceinline__ int row_in_block() { return TPR == 64 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) : 0; }
+
+// a thread's part of the row under the cursor; zeros behind D, and for a row that is not there or padding
+template <typename T, int V, int NV, int TPR>
+__device__ __forceinline__ void load_row(const View<const T>& x, const NormParams& p, const RowCursor& q, int l, vec_t<T, V> (&out)[NV]) {
+    if (q.valid) {
+        const T* row = x.row(q.b, q.t);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) out[i] = (i * TPR + l) * V < p.D ? load_raw<T, V>(row + (i * TPR + l) * V) : vec_t<T, V>{};
+    }
+}
+
+// a thread's part of gamma or beta
+template <int V, int NV, int TPR> __device__ __forceinline__ void load_param(const float* __restrict__ v, float otherwise, int D, int l, float (&out)[NV][V]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (v && (i * TPR + l) * V < D) load_vec<float, V>(v + (i * TPR + l) * V, out[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[i][j] = otherwise;
+    }
+}
+
 // thread l of a row holds columns (i TPR + l) V + j, i < NV, j < V
 template <typename T, int V, int NV, int TPR>
-__global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_forward_kernel(View<const T> x, View<T> y, NormParams p) {
-    constexpr int RPB = TPR == 1024 ? 1 : 256 / TPR;
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_forward_kernel(View<const T> x, View<T> y, NormParams p) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float red[2][TPR > 64 ? TPR / 64 : 1];       // mean and moment apart: a wave may be a reduction ahead of another
     const int l = threadIdx.x % TPR;
     float gm[NV][V], bt[NV][V];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (i * TPR + l) * V + j;
-            gm[i][j] = p.gamma && c < p.D ? p.gamma[c] : 1.f;
-            bt[i][j] = p.beta && c < p.D ? p.beta[c] : 0.f;
-        }
+    load_param<V, NV, TPR>(p.gamma, 1.f, p.D, l, gm);
+    load_param<V, NV, TPR>(p.beta, 0.f, p.D, l, bt);
     const float inv_d = 1.f / (float)p.D;
-    for (int r = blockIdx.x * RPB + threadIdx.x / TPR; r < p.rows; r += gridDim.x * RPB) {
-        const int b = r / p.T, t = r - b * p.T;
-        T* yr = y.row(b, t);
-        if (t >= valid_steps(p.lens, b, p.T)) {
+    RowCursor q(p, blockIdx.x * RPB + row_in_block<TPR>(), gridDim.x * RPB);
+    vec_t<T, V> next[NV];
+    load_row<T, V, NV, TPR>(x, p, q, l, next);
+    while (q.r < p.rows) {
+        const int r = q.r;
+        T* yr = y.row(q.b, q.t);
+        const bool valid = q.valid;
+        float v[NV][V], s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) widen<T, V>(next[i], v[i]);
+        q.advance(p);
+        load_row<T, V, NV, TPR>(x, p, q, l, next);
+        if (!valid) {
             const float zero[V] = {};
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -75,32 +116,23 @@ __global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_forward_kernel(Vi
             if (l == 0) { p.mean[r] = 0.f; p.inv_std[r] = 0.f; }
             continue;
         }
-        const T* xr = x.row(b, t);
-        float v[NV][V], s[1] = {0.f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if ((i * TPR + l) * V < p.D) load_vec<T, V>(xr + (i * TPR + l) * V, v[i]);
-            else
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = 0.f;
-        }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) s[0] += v[i][j];
         row_sums<TPR, 1>(s, red[0]);
         const float mean = s[0] * inv_d;
-        float q[1] = {0.f};
+        float m2[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float d = (i * TPR + l) * V + j < p.D ? v[i][j] - mean : 0.f;
                 v[i][j] = d;
-                q[0] += d * d;
+                m2[0] += d * d;
             }
-        row_sums<TPR, 1>(q, red[1]);
-        const float inv = 1.f / sqrtf(q[0] * inv_d + p.eps);
+        row_sums<TPR, 1>(m2, red[1]);
+        const float inv = 1.f / sqrtf(m2[0] * inv_d + p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float o[V];
@@ -113,47 +145,59 @@ __global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_forward_kernel(Vi
 }
 
 template <typename T, int V, int NV, int TPR>
-__global__ __launch_bounds__(TPR == 1024 ? 1024 : 256) void ln_backward_kernel(View<const T> x, View<const T> dy, View<T> dx, NormParams p) {
-    constexpr int RPB = TPR == 1024 ? 1 : 256 / TPR;
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_backward_kernel(View<const T> x, View<const T> dy, View<T> dx, NormParams p) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     constexpr int NW = TPR > 64 ? TPR / 64 : 1;
     __shared__ float red[2][2 * NW];                         // alternating rows: one barrier per row is then enough
     __shared__ float comb[TPR == 64 ? 2 * 64 * NV * V : 1];
     const int l = threadIdx.x % TPR;
+    // 1024 threads have 128 registers each: gamma is then read again for every row and the next row's loads wait
+    constexpr bool AHEAD = TPR < 1024;
     float gm[NV][V], dg[NV][V], db[NV][V];
+    if (AHEAD) load_param<V, NV, TPR>(p.gamma, 1.f, p.D, l, gm);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (i * TPR + l) * V + j;
-            gm[i][j] = p.gamma && c < p.D ? p.gamma[c] : 1.f;
             dg[i][j] = 0.f;
             db[i][j] = 0.f;
         }
     const float inv_d = 1.f / (float)p.D;
     int turn = 0;
-    for (int r = blockIdx.x * RPB + threadIdx.x / TPR; r < p.rows; r += gridDim.x * RPB) {
-        const int b = r / p.T, t = r - b * p.T;
-        T* dxr = dx.row(b, t);
-        if (t >= valid_steps(p.lens, b, p.T)) {
+    RowCursor q(p, blockIdx.x * RPB + row_in_block<TPR>(), gridDim.x * RPB);
+    vec_t<T, V> xn[NV], gn[NV];
+    if (AHEAD) {
+        load_row<T, V, NV, TPR>(x, p, q, l, xn);
+        load_row<T, V, NV, TPR>(dy, p, q, l, gn);
+    }
+    while (q.r < p.rows) {
+        const int r = q.r;
+        T* dxr = dx.row(q.b, q.t);
+        const bool valid = q.valid;
+        float xh[NV][V], g[NV][V];
+        if (!AHEAD) {
+            load_row<T, V, NV, TPR>(x, p, q, l, xn);
+            load_row<T, V, NV, TPR>(dy, p, q, l, gn);
+            load_param<V, NV, TPR>(p.gamma, 1.f, p.D, l, gm);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            widen<T, V>(xn[i], xh[i]);
+            widen<T, V>(gn[i], g[i]);
+        }
+        q.advance(p);
+        if (AHEAD) {
+            load_row<T, V, NV, TPR>(x, p, q, l, xn);
+            load_row<T, V, NV, TPR>(dy, p, q, l, gn);
+        }
+        if (!valid) {
             const float zero[V] = {};
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if ((i * TPR + l) * V < p.D) store_vec<T, V>(dxr + (i * TPR + l) * V, zero);
             continue;
         }
-        const T* xr = x.row(b, t);
-        const T* gr = dy.row(b, t);
         const float mean = p.mean[r], inv = p.inv_std[r];
-        float xh[NV][V], g[NV][V];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if ((i * TPR + l) * V < p.D) {
-                load_vec<T, V>(xr + (i * TPR + l) * V, xh[i]);
-                load_vec<T, V>(gr + (i * TPR + l) * V, g[i]);
-            } else
-#pragma unroll
-                for (int j = 0; j < V; ++j) { xh[i][j] = mean; g[i][j] = 0.f; }
-        }
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -211,8 +255,18 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + cl;
     float a = 0.f;
-    if (c < total)
-        for (int k = rl; k < parts; k += 32) a += ws[(int64_t)k * stride + c];
+    if (c < total) {
+        const float* src = ws + c;
+        int k = rl;
+        for (; k + 32 * 7 < parts; k += 32 * 8) {      // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = src[(int64_t)(k + 32 * i) * stride];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a += v[i];
+        }
+        for (; k < parts; k += 32) a += src[(int64_t)k * stride];
+    }
     red[rl][cl] = a;
     __syncthreads();
     if (rl == 0 && c < total) {
@@ -232,9 +286,15 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 
 constexpr int kMaxNormChannels = 16 * 1024;
 
-// backward: how many workgroups leave a partial row.  Two per CU hide each other's waits; more only add partial rows to sum
-int norm_parts(int64_t rows, int rows_per_block) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, 1024)); }
-int norm_tpr(int D) { return D <= 16 * 64 ? 64 : (D <= 16 * 256 ? 256 : 1024); }
+constexpr int kNormBlocks = 1024;      // forward: four persistent workgroups per CU
+// backward: workgroups, each of which leaves a partial row -- as many as are resident at once: one more round of fewer costs more than
+// idle CUs (32768 x 4096 bf16: 768 workgroups 168 us, 1024 184 us; 20800 x 2000: 1024 58 us, 768 65 us)
+int norm_parts(int64_t rows, int D, int tpr) {
+    const int most = tpr == 64 ? 768 : (tpr == 256 ? (D <= 8 * 256 ? 1024 : 768) : 256);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(tpr == 64 ? (rows + 3) / 4 : rows, most));
+}
+// forward a wave keeps rows of up to 2048 columns (no barriers); the backward pass adds gamma's and beta's gradients beside them
+int norm_tpr(int D, bool bwd) { return D <= (bwd ? 16 : 32) * 64 ? 64 : (D <= 16 * 256 ? 256 : (D <= 16 * 512 ? 512 : 1024)); }
 
 int check(const adn_norm_args* a, bool backward, const char* who) {
     ADN_CHECK(a, ADN_ERR_INVALID, std::string(who) + ": null arguments");
@@ -253,27 +313,30 @@ int check(const adn_norm_args* a, bool backward, const char* who) {
 
 // dispatch over element type, vector width and threads per row
 template <typename T, int V, bool BWD> int launch(const adn_norm_args& a, const NormParams& p, hipStream_t s) {
-    const int tpr = norm_tpr(p.D);
+    const int tpr = norm_tpr(p.D, BWD);
     const int rpb = tpr == 64 ? 4 : 1;
-    const int grid = BWD ? norm_parts(p.rows, rpb) : (int)std::min<int64_t>(((int64_t)p.rows + rpb - 1) / rpb, 4096);
+    const int grid = BWD ? norm_parts(p.rows, p.D, tpr) : (int)std::min<int64_t>(((int64_t)p.rows + rpb - 1) / rpb, kNormBlocks);
     const View<const T> x = cview<T>(a.x);
-    auto go = [&](auto fwd, auto bwd, int threads) {
-        if constexpr (BWD) hipLaunchKernelGGL(bwd, dim3(grid), dim3(threads), 0, s, x, cview<T>(a.dy), view<T>(a.dx), p);
-        else hipLaunchKernelGGL(fwd, dim3(grid), dim3(threads), 0, s, x, view<T>(a.y), p);
-    };
     constexpr int NV = 16 / V;
-#define ADN_LN_GO(TPR_, NV_) go(ln_forward_kernel<T, V, NV_, TPR_>, ln_backward_kernel<T, V, NV_, TPR_>, TPR_ == 1024 ? 1024 : 256)
+#define ADN_LN_GO(TPR_, NV_)                                                                                                                  \
+    do {                                                                                                                                      \
+        if constexpr (BWD)                                                                                                                    \
+            hipLaunchKernelGGL((ln_backward_kernel<T, V, NV_, TPR_>), dim3(grid), dim3(TPR_ < 256 ? 256 : TPR_), 0, s, x, cview<T>(a.dy), view<T>(a.dx), p); \
+        else                                                                                                                                  \
+            hipLaunchKernelGGL((ln_forward_kernel<T, V, NV_, TPR_>), dim3(grid), dim3(TPR_ < 256 ? 256 : TPR_), 0, s, x, view<T>(a.y), p);   \
+    } while (0)
     if (tpr == 64) {
         if (p.D <= 64 * V) ADN_LN_GO(64, 1);
         else if (p.D <= 64 * 8) ADN_LN_GO(64, (8 / V));
-        else ADN_LN_GO(64, NV);
+        else if (BWD || p.D <= 64 * 16) ADN_LN_GO(64, NV);
+        else if constexpr (!BWD) ADN_LN_GO(64, (32 / V));
     } else if (tpr == 256) {
         if (p.D <= 256 * 8) ADN_LN_GO(256, (8 / V));
         else ADN_LN_GO(256, NV);
-    } else {
-        if (p.D <= 1024 * 8) ADN_LN_GO(1024, (8 / V));
-        else ADN_LN_GO(1024, NV);
-    }
+    } else if (tpr == 512)
+        ADN_LN_GO(512, NV);
+    else
+        ADN_LN_GO(1024, NV);
 #undef ADN_LN_GO
     ADN_HIP_CHECK(hipGetLastError());
     return ADN_OK;
@@ -282,7 +345,7 @@ template <typename T, int V, bool BWD> int launch(const adn_norm_args& a, const 
 template <bool BWD> int run(const adn_norm_args& a, const NormParams& p, hipStream_t s) {
     const bool bf = a.dtype == ADN_DTYPE_BF16;
     const int e = bf ? 2 : 4;
-    const bool al = a.channels * e % 16 == 0 && seq_aligned(a.x, e, 16) && (BWD ? seq_aligned(a.dy, e, 16) && seq_aligned(a.dx, e, 16) : seq_aligned(a.y, e, 16));
+    const bool al = a.channels * e % 16 == 0 && ptr_aligned(a.gamma, 16) && (BWD || ptr_aligned(a.beta, 16)) && seq_aligned(a.x, e, 16) && (BWD ? seq_aligned(a.dy, e, 16) && seq_aligned(a.dx, e, 16) : seq_aligned(a.y, e, 16));
     if (bf) return al ? launch<__bf16, 8, BWD>(a, p, s) : launch<__bf16, 1, BWD>(a, p, s);
     return al ? launch<float, 4, BWD>(a, p, s) : launch<float, 1, BWD>(a, p, s);
 }
@@ -318,7 +381,7 @@ extern "C" void adn_op_abi_sizes(int32_t out[3]) {
 extern "C" int64_t adn_op_layer_norm_workspace(int32_t batch, int32_t steps, int32_t channels) {
     if (batch < 0 || steps < 0 || channels < 1 || channels > kMaxNormChannels) return -1;
     const int64_t rows = (int64_t)batch * steps;
-    return rows ? (int64_t)norm_parts(rows, norm_tpr(channels) == 64 ? 4 : 1) * 2 * channels : 0;
+    return rows ? (int64_t)norm_parts(rows, channels, norm_tpr(channels, true)) * 2 * channels : 0;
 }
 
 extern "C" int adn_op_layer_norm_forward(const adn_norm_args* a, void* hip_stream) {

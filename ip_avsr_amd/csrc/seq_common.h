@@ -24,9 +24,11 @@ template <typename T, int V> __device__ __forceinline__ void widen(const vec_t<T
     for (int i = 0; i < V; ++i) out[i] = (float)v[i];
 }
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* __restrict__ p, float* out) {
-    const vec_t<T, V> v = *reinterpret_cast<const vec_t<T, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+    if constexpr (sizeof(T) * V > 16) {      // 16 bytes at a time: no wider alignment is asked for
+        load_vec<T, V / 2>(p, out);
+        load_vec<T, V / 2>(p + V / 2, out + V / 2);
+    } else
+        widen<T, V>(load_raw<T, V>(p), out);
 }
 // rounds to nearest even where T is bfloat16: the one rounding of a result
 template <typename T, int V> __device__ __forceinline__ void store_vec(T* __restrict__ p, const float* in) {
