@@ -631,6 +631,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
+// sum of n values `stride` apart, in order, eight loads in flight
+__device__ __forceinline__ float strided_sum(const float* __restrict__ src, int64_t stride, int n) {
+    float a = 0.f;
+    int k = 0;
+    for (; k + 8 <= n; k += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = src[(k + i) * stride];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a += v[i];
+    }
+    for (; k < n; ++k) a += src[k * stride];
+    return a;
+}
+
 // the second launch of the backward pass: workgroups [0, nb_bc) add dB and dC over the workgroups of a group, the others dA, dD and
 // the bias' gradient over the groups of utterances
 template <typename T, int NS>
@@ -648,7 +663,7 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
         float a = 0.f;
         if (t < valid_steps(p.lens, b, p.T)) {
             const float* src = p.part_bc + (((int64_t)b * p.nseg + t / SEG) * p.G + g) * STAGE + (t % SEG) * 8 * NS + which * 4 * NS + n;
-            for (int k = 0; k < p.bpg; ++k) a += src[(int64_t)k * p.B * p.nseg * p.G * STAGE];
+            a = strided_sum(src, (int64_t)p.B * p.nseg * p.G * STAGE, p.bpg);
         }
         (which ? dC : dB)[o] = (T)a;
         return;
@@ -664,8 +679,7 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
         at = (m / 4 * 64 + lane) * 4 + m % 4;
     } else
         at = 64 * P + (i - da >= p.D ? WC : 0) + cw;
-    float a = 0.f;
-    for (int k = 0; k < p.nbg * p.chunks; ++k) a += p.part_a[row + at + k * stride];
+    const float a = strided_sum(p.part_a + row + at, stride, p.nbg * p.chunks);
     if (i < da) dA[i] = a;
     else if (i - da < p.D) dD[c] = a;
     else dbias[c] = a;
