@@ -685,8 +685,9 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
     else dbias[c] = a;
 }
 
-// one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane
-template <typename T, int NS>
+// one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane; VEC: N = 4 NS and
+// everything aligned for NS values at a time.  Bound by the state's bytes, in and out
+template <typename T, int NS, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u, int64_t ldu, const T* __restrict__ delta, int64_t ldd, const T* __restrict__ bm,
                                                         int64_t ldb, const T* __restrict__ cm, int64_t ldc, const T* __restrict__ z, int64_t ldz,
                                                         T* __restrict__ y, int64_t ldy, ScanParams p) {
@@ -701,17 +702,33 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u,
     float* h = p.state_out + item * p.N;
     const T* br = bm + b * ldb + (int64_t)g * p.N;
     const T* cr = cm + b * ldc + (int64_t)g * p.N;
-    float acc = 0.f;
+    float acc = 0.f, hv[NS], av[NS], bv[NS], cv[NS];
+    if constexpr (VEC) {
+        load_vec<float, NS>(h + ng * NS, hv);
+        load_vec<float, NS>(p.A + (int64_t)c * p.N + ng * NS, av);
+        load_vec<T, NS>(br + ng * NS, bv);
+        load_vec<T, NS>(cr + ng * NS, cv);
+    } else {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        const int n = ng * NS + j;
-        if (n < p.N) {
-            const float a = __builtin_amdgcn_exp2f(dt * (p.A[(int64_t)c * p.N + n] * kLog2e));
-            const float hv = fmaf(a, h[n], dtu * (float)br[n]);
-            h[n] = hv;
-            acc = fmaf(hv, (float)cr[n], acc);
+        for (int j = 0; j < NS; ++j) {
+            const int n = ng * NS + j;
+            const bool on = n < p.N;
+            hv[j] = on ? h[n] : 0.f;
+            av[j] = on ? p.A[(int64_t)c * p.N + n] : 0.f;
+            bv[j] = on ? (float)br[n] : 0.f;
+            cv[j] = on ? (float)cr[n] : 0.f;
         }
     }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        hv[j] = fmaf(__builtin_amdgcn_exp2f(dt * (av[j] * kLog2e)), hv[j], dtu * bv[j]);
+        acc = fmaf(hv[j], cv[j], acc);
+    }
+    if constexpr (VEC) store_vec<float, NS>(h + ng * NS, hv);
+    else
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+            if (ng * NS + j < p.N) h[ng * NS + j] = hv[j];
     acc += dpp<kQuadXor1>(acc);
     acc += dpp<kQuadXor2>(acc);
     if (ng == 0) {
@@ -846,9 +863,16 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
 
 template <typename T, int NS> int step(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
     const int64_t items = (int64_t)p.B * p.D;
-    hipLaunchKernelGGL((scan_step_kernel<T, NS>), dim3((unsigned)((items + 63) / 64)), dim3(256), 0, s, static_cast<const T*>(a.u.data), a.u.stride_b,
-                       static_cast<const T*>(a.delta.data), a.delta.stride_b, static_cast<const T*>(a.b.data), a.b.stride_b, static_cast<const T*>(a.c.data),
-                       a.c.stride_b, static_cast<const T*>(a.z.data), a.z.stride_b, static_cast<T*>(a.y.data), a.y.stride_b, p);
+    const int e = sizeof(T);
+    const auto rows = [&](const adn_seq& t) { return ptr_aligned(t.data, NS * e) && t.stride_b % NS == 0; };
+    const bool vec = p.N == 4 * NS && ptr_aligned(p.A, 16) && ptr_aligned(p.state_out, 16) && rows(a.b) && rows(a.c);
+#define ADN_SCAN_GO(VEC)                                                                                                                           \
+    hipLaunchKernelGGL((scan_step_kernel<T, NS, VEC>), dim3((unsigned)((items + 63) / 64)), dim3(256), 0, s, static_cast<const T*>(a.u.data), a.u.stride_b, \
+                       static_cast<const T*>(a.delta.data), a.delta.stride_b, static_cast<const T*>(a.b.data), a.b.stride_b, static_cast<const T*>(a.c.data), \
+                       a.c.stride_b, static_cast<const T*>(a.z.data), a.z.stride_b, static_cast<T*>(a.y.data), a.y.stride_b, p)
+    if (vec) ADN_SCAN_GO(true);
+    else ADN_SCAN_GO(false);
+#undef ADN_SCAN_GO
     ADN_HIP_CHECK(hipGetLastError());
     return ADN_OK;
 }

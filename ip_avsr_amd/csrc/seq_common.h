@@ -32,10 +32,16 @@ template <typename T, int V> __device__ __forceinline__ void load_vec(const T* _
 }
 // rounds to nearest even where T is bfloat16: the one rounding of a result
 template <typename T, int V> __device__ __forceinline__ void store_vec(T* __restrict__ p, const float* in) {
-    vec_t<T, V> v;
+    if constexpr (sizeof(T) * V > 16) {
+        store_vec<T, V / 2>(p, in);
+        store_vec<T, V / 2>(p + V / 2, in + V / 2);
+        return;
+    } else {
+        vec_t<T, V> v;
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (T)in[i];
-    *reinterpret_cast<vec_t<T, V>*>(p) = v;
+        for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+        *reinterpret_cast<vec_t<T, V>*>(p) = v;
+    }
 }
 
 // frames of utterance b that are no padding; values outside [0, T] are clamped
