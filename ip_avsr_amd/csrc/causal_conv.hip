@@ -56,10 +56,10 @@ __device__ __forceinline__ void frames(const View<const T>& x, const ConvParams&
 // workgroup: 64 lanes x V channels, 4 waves = 4 runs
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void conv_forward_kernel(View<const T> x, View<T> y, ConvParams p) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    const int item = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);      // B runs < 2^31 - 4
     const int c = ((int)blockIdx.y * 64 + (int)(threadIdx.x & 63)) * V;
-    if (item >= (int64_t)p.B * p.runs || c >= p.C) return;
-    const int b = (int)(item / p.runs), ri = (int)(item - (int64_t)b * p.runs);
+    if (item >= p.B * p.runs || c >= p.C) return;
+    const int b = item / p.runs, ri = item - b * p.runs;
     const int t0 = ri * p.run, t1 = min(p.T, t0 + p.run), len = valid_steps(p.lens, b, p.T);
     float w[K][V], bias[V];
 #pragma unroll
@@ -120,9 +120,9 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
 #pragma unroll
         for (int j = 0; j < V; ++j) bias[j] = 0.f;
         if (p.bias) load_vec<float, V>(p.bias + c, bias);
-        const int64_t items = (int64_t)p.B * p.runs;
-        for (int64_t item = (int64_t)blockIdx.x * 4 + wv; item < items; item += (int64_t)p.parts * 4) {
-            const int b = (int)(item / p.runs), ri = (int)(item - (int64_t)b * p.runs);
+        const int items = p.B * p.runs;                        // < 2^31 - 65536, and a step is at most 4096: no overflow
+        for (int item = (int)blockIdx.x * 4 + wv; item < items; item += p.parts * 4) {
+            const int b = item / p.runs, ri = item - b * p.runs;
             const int t0 = ri * p.run, t1 = min(p.T, t0 + p.run), len = valid_steps(p.lens, b, p.T);
             const auto gradients = [&](int t, vec_t<T, V> (&out)[kConvChunk]) {
                 if (t + kConvChunk <= len) {
@@ -345,7 +345,7 @@ extern "C" int adn_op_causal_conv_forward(const adn_conv_args* a, void* hip_stre
                     ptr_aligned(a->state, 16) && ptr_aligned(a->state_out, 16);
     p.run = run_length(p.B, std::max(p.T, 1), cdiv(p.C, 64 * (al ? v : 1)));
     p.runs = std::max(1, cdiv(p.T, p.run));      // (no frames: the history is still handed on)
-    ADN_CHECK((int64_t)p.B * p.runs < (int64_t)1 << 32, ADN_ERR_INVALID, "adn_op_causal_conv_forward: batch too large");
+    ADN_CHECK((int64_t)p.B * p.runs < ((int64_t)1 << 31) - 65536, ADN_ERR_INVALID, "adn_op_causal_conv_forward: batch too large");
     if (a->dtype == ADN_DTYPE_BF16) return al ? launch<__bf16, 8, kForward>(*a, p, s) : launch<__bf16, 1, kForward>(*a, p, s);
     return al ? launch<float, 4, kForward>(*a, p, s) : launch<float, 1, kForward>(*a, p, s);
 }
@@ -365,6 +365,7 @@ extern "C" int adn_op_causal_conv_backward(const adn_conv_args* a, void* hip_str
         const int v = conv_bwd_vec(*a);
         p.parts = conv_parts(p.B, std::max(p.T, 1), p.C, v, &p.run);
         p.runs = std::max(1, cdiv(p.T, p.run));
+        ADN_CHECK((int64_t)p.B * p.runs < ((int64_t)1 << 31) - 65536, ADN_ERR_INVALID, "adn_op_causal_conv_backward: batch too large");
         p.part = a->workspace;
         if (a->dtype == ADN_DTYPE_BF16) ADN_TRY((v == 1 ? launch<__bf16, 1, kBackward>(*a, p, s) : launch<__bf16, kConvBwdV, kBackward>(*a, p, s)));
         else ADN_TRY((v == 1 ? launch<float, 1, kBackward>(*a, p, s) : launch<float, kConvBwdV, kBackward>(*a, p, s)));

@@ -691,15 +691,15 @@ template <typename T, int NS, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u, int64_t ldu, const T* __restrict__ delta, int64_t ldd, const T* __restrict__ bm,
                                                         int64_t ldb, const T* __restrict__ cm, int64_t ldc, const T* __restrict__ z, int64_t ldz,
                                                         T* __restrict__ y, int64_t ldy, ScanParams p) {
-    const int64_t item = (int64_t)blockIdx.x * 64 + threadIdx.x / 4;
+    const unsigned item = blockIdx.x * 64 + threadIdx.x / 4;      // B D < 2^31
     const int ng = threadIdx.x & 3;
-    if (item >= (int64_t)p.B * p.D) return;              // whole quads leave
-    const int b = (int)(item / p.D), c = (int)(item - (int64_t)b * p.D), g = c / p.Dg;
+    if (item >= (unsigned)p.B * (unsigned)p.D) return;             // whole quads leave
+    const int b = (int)(item / (unsigned)p.D), c = (int)(item - (unsigned)b * (unsigned)p.D), g = p.G == 1 ? 0 : c / p.Dg;
     const float uv = (float)u[b * ldu + c];
     float dt = (float)delta[b * ldd + c] + (p.dbias ? p.dbias[c] : 0.f);
     if (p.softplus) dt = softplusf(dt);
     const float dtu = dt * uv;
-    float* h = p.state_out + item * p.N;
+    float* h = p.state_out + (int64_t)item * p.N;
     const T* br = bm + b * ldb + (int64_t)g * p.N;
     const T* cr = cm + b * ldc + (int64_t)g * p.N;
     float acc = 0.f, hv[NS], av[NS], bv[NS], cv[NS];
