@@ -134,6 +134,10 @@ template <typename T> struct Walk {
     __device__ __forceinline__ T* at(int t0) const { return reinterpret_cast<T*>(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame) + off); }
 };
 
+// LDS reads stay on their side of this point: a frame's B and C are read while the frame before is computed.  Without it the compiler
+// puts each read right before its use, and a lone wave on its SIMD waits for every one
+__device__ __forceinline__ void hold_reads() { __builtin_amdgcn_sched_barrier(0x277); }
+
 template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p, int b, int seg, int ctile) {
     return (((int64_t)b * p.nseg + seg) * p.ctiles + ctile) * 64 * P;
 }
@@ -229,14 +233,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             total += dt[i];
         }
         if (k0 + 1 < n) fetch(BACK ? seg - 1 : seg + 1);
+        float mn1[NS];
+        load_vec<float, NS>(buf + (BACK ? SEG - 1 : 0) * 4 * NS + l.ng * NS, mn1);
 #pragma unroll
         for (int ii = 0; ii < Q; ++ii) {
             const int i = BACK ? Q - 1 - ii : ii;
 #pragma unroll
             for (int tt = 0; tt < TQ; ++tt) {
-                const int tp = BACK ? TQ - 1 - tt : tt;
+                const int tp = BACK ? TQ - 1 - tt : tt, at = i * TQ + tp, after = BACK ? at - 1 : at + 1;
                 float mv[NS];
-                load_vec<float, NS>(buf + (i * TQ + tp) * 4 * NS + l.ng * NS, mv);
+#pragma unroll
+                for (int j = 0; j < NS; ++j) mv[j] = mn1[j];
+                if (after >= 0 && after < SEG) load_vec<float, NS>(buf + after * 4 * NS + l.ng * NS, mn1);
+                hold_reads();
 #pragma unroll
                 for (int k = 0; k < NC; ++k) {
                     const float dtk = bcast(dt[i], tp * NC + k), ink = bcast(in[i], tp * NC + k);
@@ -338,15 +347,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
                 store_vec<float, 4>(ck + m * 256, v);
             }
         }
+        float bn[NS], cn[NS];
+        load_vec<float, NS>(buf + l.ng * NS, bn);
+        load_vec<float, NS>(buf + 4 * NS + l.ng * NS, cn);
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
             const float dtu = dt[i] * uc[i];
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int tp = 0; tp < TQ; ++tp) {
+                const int after = i * TQ + tp + 1;
                 float bv[NS], cv[NS];
-                load_vec<float, NS>(buf + (i * TQ + tp) * 8 * NS + l.ng * NS, bv);
-                load_vec<float, NS>(buf + (i * TQ + tp) * 8 * NS + 4 * NS + l.ng * NS, cv);
+#pragma unroll
+                for (int j = 0; j < NS; ++j) { bv[j] = bn[j]; cv[j] = cn[j]; }
+                if (after < SEG) {
+                    load_vec<float, NS>(buf + after * 8 * NS + l.ng * NS, bn);
+                    load_vec<float, NS>(buf + after * 8 * NS + 4 * NS + l.ng * NS, cn);
+                }
+                hold_reads();
 #pragma unroll
                 for (int k = 0; k < NC; ++k) {
                     const int q = tp * NC + k;
@@ -530,7 +548,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
             if (seg > s0) fetch(seg - 1);
-            float a[SEG][NC][NS], e[SEG][NC][NS];
+            float a[SEG][NC][NS], e[SEG][NC][NS], bn[NS], cn[NS];
+            load_vec<float, NS>(buf + l.ng * NS, bn);
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
                 const float dtu = dt[i] * uc[i];
@@ -538,7 +557,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int tp = 0; tp < TQ; ++tp) {
                     const int s = i * TQ + tp;
                     float bv[NS];
-                    load_vec<float, NS>(buf + s * 8 * NS + l.ng * NS, bv);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) bv[j] = bn[j];
+                    load_vec<float, NS>(buf + min(s + 1, SEG - 1) * 8 * NS + l.ng * NS, bn);
+                    if (s + 1 == SEG) load_vec<float, NS>(buf + s * 8 * NS + 4 * NS + l.ng * NS, cn);
+                    hold_reads();
 #pragma unroll
                     for (int k = 0; k < NC; ++k) {
                         const float dtk = bcast(dt[i], tp * NC + k), dtuk = bcast(dtu, tp * NC + k);
@@ -561,8 +584,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int tp = TQ - 1; tp >= 0; --tp) {
                     const int s = i * TQ + tp;
                     float bv[NS], cv[NS], sums[2 * NS];
-                    load_vec<float, NS>(buf + s * 8 * NS + l.ng * NS, bv);
-                    load_vec<float, NS>(buf + s * 8 * NS + 4 * NS + l.ng * NS, cv);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) { bv[j] = bn[j]; cv[j] = cn[j]; }
+                    if (s > 0) {
+                        load_vec<float, NS>(buf + (s - 1) * 8 * NS + l.ng * NS, bn);
+                        load_vec<float, NS>(buf + (s - 1) * 8 * NS + 4 * NS + l.ng * NS, cn);
+                    }
+                    hold_reads();
 #pragma unroll
                     for (int j = 0; j < 2 * NS; ++j) sums[j] = 0.f;
 #pragma unroll
