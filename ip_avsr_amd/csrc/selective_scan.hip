@@ -796,7 +796,7 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G, bool bwd) {
     const int64_t waves = B * q.tpg * G;
     q.chunks = 1;
     if (B > 0 && waves <= (bwd ? 1024 : 768) && q.nseg >= 2 * kMinPiece)
-        q.chunks = (int)std::min<int64_t>(q.nseg / kMinPiece, ((bwd ? 2048 : 4096) + waves - 1) / waves);
+        q.chunks = (int)std::min<int64_t>(q.nseg / kMinPiece, (4096 + waves - 1) / waves);
     q.spc = std::max(1, cdiv(q.nseg, q.chunks));
     q.chunks = std::max(1, cdiv(q.nseg, q.spc));
     q.local = q.chunks > 1 ? B * q.chunks * q.ctiles * 64 * P : 0;
