@@ -23,6 +23,7 @@
 // over all frames of a workgroup's utterances.  All sums run in a fixed order.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
+#include <type_traits>
 
 namespace adn {
 namespace seq {
@@ -93,10 +94,9 @@ __device__ __forceinline__ float quad_gather(const float (&v)[4], bool b0, bool 
 template <int NS> struct Place {
     static constexpr int NC = channels_per_quad(NS), SEG = segment_frames(NS), TQ = 4 / NC, WC = 16 * NC, P = NC * NS, Q = SEG / TQ;
     static constexpr int STAGE = SEG * 8 * NS, SPT = (STAGE + 255) / 256;      // values of B and C in a segment, and per thread
-    int lane, wv, ng, cl, g, ctile, c0, cend, oc, ld, otp;
+    int lane, wv, ng, cl, g, ctile, c0, cend, oc, otp;
     bool ocv, b0, b1;
-    int st_s, st_at, st_which;        // the staged value of this thread: frame, place in the row of its group, B or C
-    bool st_on;
+    int st_s, st_at, st_which;        // the staged value of this thread: frame (none: far behind any), place in the row of its group, B or C
     __device__ __forceinline__ Place(const ScanParams& p, int cblk) {
         lane = threadIdx.x & 63;
         wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
@@ -110,29 +110,47 @@ template <int NS> struct Place {
         oc = c0 + ng % NC;                          // the channel and, below, the frame of the quad that this lane owns
         otp = ng / NC;
         ocv = oc < cend;
-        ld = min(oc, cend - 1);                     // a lane without a channel loads the last one's and drops it
         b0 = ng & 1;
         b1 = ng >> 1;
         st_s = (int)threadIdx.x / (8 * NS);
         st_which = ((int)threadIdx.x / (4 * NS)) & 1;
         const int n = (int)threadIdx.x % (4 * NS);
-        st_on = (int)threadIdx.x < STAGE && n < p.N;
-        st_at = g * p.N + min(n, p.N - 1);
+        st_at = g * p.N + n;
+        if ((int)threadIdx.x >= STAGE || n >= p.N) st_s = 1 << 30;
     }
 };
 static_assert(Place<1>::SPT == 1 && Place<2>::SPT == 1 && Place<4>::SPT == 1 && Place<8>::SPT == 1, "one staged value per thread");
 
-// a (B, T, D) tensor as a wave walks one utterance: a uniform pointer to the segment and a 32-bit offset per lane (check() holds the
-// frame stride below 2^28)
+// a (B, T, D) tensor as a wave walks one utterance: buffer accesses from a uniform base at a segment's first frame, with a 32-bit offset
+// per lane (check() holds the frame stride below 2^26).  A lane without a channel, or without a frame, gets the offset that the bounds
+// check turns away: its load is 0, its store is dropped, and no branch stands between the loads in flight
+constexpr uint32_t kNowhere = 0x80000000u;
 template <typename T> struct Walk {
     const char* p;
     uint32_t frame;                    // bytes between frames
-    uint32_t off;
-    __device__ __forceinline__ Walk(const View<T>& v, int b, int frame_of_lane, int c)
-        : p(reinterpret_cast<const char*>(v.p + b * v.sb)), frame((uint32_t)v.st * (uint32_t)sizeof(T)), off((uint32_t)((uint32_t)frame_of_lane * (uint32_t)v.st + (uint32_t)c) * (uint32_t)sizeof(T)) {}
-    // the lane's element, t0 frames on
-    __device__ __forceinline__ T* at(int t0) const { return reinterpret_cast<T*>(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame) + off); }
+    uint32_t off;                      // of the lane's first frame in a segment
+    __device__ __forceinline__ Walk(const View<T>& v, int b, int frame_of_lane, int c, bool on)
+        : p(reinterpret_cast<const char*>(v.p + b * v.sb)), frame((uint32_t)v.st * (uint32_t)sizeof(T)),
+          off(on ? (uint32_t)frame_of_lane * frame + (uint32_t)c * (uint32_t)sizeof(T) : kNowhere) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t base(int t0) const {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame), 0, 0x7FFFFFFF, 0x00027000);
+    }
+    // `ahead` frames behind the lane's first; `on`: whether there is such a frame
+    __device__ __forceinline__ uint32_t at(int ahead, bool on) const { return on ? off + (uint32_t)ahead * frame : kNowhere; }
+    // without bounds, for the frames behind the last segment
+    __device__ __forceinline__ T* to(int t0) const { return reinterpret_cast<T*>(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame) + off); }
 };
+__device__ __forceinline__ float raw_to_float(uint32_t v, float) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ float raw_to_float(uint32_t v, __bf16) { return __builtin_bit_cast(float, v << 16); }
+// the bits of an element (a bfloat16 in the lower half)
+template <typename T> __device__ __forceinline__ uint32_t buf_load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    if constexpr (sizeof(T) == 2) return (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+}
+template <typename T> __device__ __forceinline__ void buf_store(__amdgpu_buffer_rsrc_t r, uint32_t off, float v) {
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)v), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, off, 0, 0);
+}
 
 // LDS reads stay on their side of this point: a frame's B and C are read while the frame before is computed.  Without it the compiler
 // puts each read right before its use, and a lone wave on its SIMD waits for every one
@@ -187,52 +205,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             h[k][j] = !BACK && on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
     const float bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
-    const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld);
+    const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv);
     const int ms = (int)threadIdx.x / (4 * NS), mn = (int)threadIdx.x % (4 * NS);
     const bool mon = (int)threadIdx.x < ROWS && mn < p.N;
-    const Walk<const T> wm(m, b, min(ms, SEG - 1), l.g * p.N + min(mn, p.N - 1));
-    T un[Q], xn[Q], zn[Q], st;
-    auto fetch = [&](int seg) {
-        const int t0 = seg * SEG;
-        if (t0 + SEG <= len) {
-            st = *wm.at(t0);
+    const Walk<const T> wm(m, b, ms, l.g * p.N + mn, mon);
+    uint32_t un[2][Q], xn[2][Q], zn[2][Q], st[2];
+    const auto fetch = [&](int k0, auto set) {          // the k0-th segment of the piece; none: the last one again
+        constexpr int R = decltype(set)::value;
+        const int k = min(k0, s1 - s0 - 1), t0 = (BACK ? s1 - 1 - k : s0 + k) * SEG;
+        const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0);
+        st[R] = buf_load<T>(wm.base(t0), wm.at(0, ms < len - t0));
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                un[i] = *wu.at(t0 + i * TQ);
-                xn[i] = *wx.at(t0 + i * TQ);
-                if (BACK && GATED) zn[i] = *wz.at(t0 + i * TQ);
-            }
-        } else {
-            st = t0 + min(ms, SEG - 1) < len ? *wm.at(t0) : (T)0.f;
-#pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const bool on = t0 + i * TQ + l.otp < len;
-                un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
-                xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
-                if (BACK && GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
-            }
+        for (int i = 0; i < Q; ++i) {
+            const bool on = t0 + i * TQ + l.otp < len;
+            un[R][i] = buf_load<T>(ru, wu.at(i * TQ, on));
+            xn[R][i] = buf_load<T>(rx, wx.at(i * TQ, on));
+            if (BACK && GATED) zn[R][i] = buf_load<T>(rz, wz.at(i * TQ, on));
         }
     };
     float total = 0.f;
     const int n = s1 - s0;
-    fetch(BACK ? s1 - 1 : s0);
-    for (int k0 = 0; k0 < n; ++k0) {
+    const auto segment = [&](int k0, auto set) {
+        constexpr int R = decltype(set)::value;
         const int seg = BACK ? s1 - 1 - k0 : s0 + k0, t0 = seg * SEG;
-        float* buf = bc[k0 & 1];
-        if ((int)threadIdx.x < ROWS) buf[threadIdx.x] = mon ? (float)st : 0.f;
+        float* buf = bc[R];
+        if ((int)threadIdx.x < ROWS) buf[threadIdx.x] = raw_to_float(st[R], T{});
         __syncthreads();
         float in[Q], dt[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            const float x = l.ocv ? (float)xn[i] + bias : 0.f;
+            const float x = raw_to_float(xn[R][i], T{}) + bias;
             dt[i] = p.softplus ? softplusf(x) : x;
             if (t0 + SEG > len) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;
-            in[i] = l.ocv ? (float)un[i] : 0.f;
+            in[i] = raw_to_float(un[R][i], T{});
             if (!BACK) in[i] *= dt[i];
-            else if (GATED) { const float zc = l.ocv ? (float)zn[i] : 0.f; in[i] *= zc * sigmoidf(zc); }
+            else if (GATED) { const float zc = raw_to_float(zn[R][i], T{}); in[i] *= zc * sigmoidf(zc); }
             total += dt[i];
         }
-        if (k0 + 1 < n) fetch(BACK ? seg - 1 : seg + 1);
+        fetch(k0 + 2, set);
         float mn1[NS];
         load_vec<float, NS>(buf + (BACK ? SEG - 1 : 0) * 4 * NS + l.ng * NS, mn1);
 #pragma unroll
@@ -257,6 +267,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
                 }
             }
         }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    fetch(0, even);
+    fetch(1, odd);
+    for (int k0 = 0; k0 < n; k0 += 2) {
+        segment(k0, even);
+        if (k0 + 1 < n) segment(k0 + 1, odd);
     }
     float* out = p.local + local_at<P>(p, b, chunk, l.ctile) + l.lane * 4;
 #pragma unroll
@@ -295,48 +313,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     if (s0 < nv)
         for (int c = 0; c < chunk; ++c) carry_over<NS>(p, l, b, c, A2, h);
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
-    const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld);
-    const Walk<T> wy(y, b, l.otp, l.ld);
-    const Walk<const T> wb(l.st_which ? cm : bm, b, l.st_s, l.st_at);
-    T un[Q], xn[Q], zn[Q], st;
-    auto fetch = [&](int seg) {
-        const int t0 = seg * SEG;
-        if (t0 + SEG <= len) {
-            st = *wb.at(t0);
+    const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv);
+    const Walk<T> wy(y, b, l.otp, l.oc, l.ocv);
+    const Walk<const T> wb(bm, b, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
+    // a segment's loads are issued two segments ahead, into one of two sets of registers
+    uint32_t un[2][Q], xn[2][Q], zn[2][Q], st[2];
+    const auto fetch = [&](int of, auto set) {          // behind the last segment: the last one again
+        constexpr int R = decltype(set)::value;
+        const int t0 = min(of, s1 - 1) * SEG;
+        const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0);
+        st[R] = buf_load<T>(wb.base(t0), wb.at(0, l.st_s < len - t0)) | buf_load<T>(wc.base(t0), wc.at(0, l.st_s < len - t0));
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                un[i] = *wu.at(t0 + i * TQ);
-                xn[i] = *wx.at(t0 + i * TQ);
-                if (GATED) zn[i] = *wz.at(t0 + i * TQ);
-            }
-        } else {
-            st = t0 + l.st_s < len ? *wb.at(t0) : (T)0.f;
-#pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const bool on = t0 + i * TQ + l.otp < len;
-                un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
-                xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
-                if (GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
-            }
+        for (int i = 0; i < Q; ++i) {
+            const bool on = t0 + i * TQ + l.otp < len;
+            un[R][i] = buf_load<T>(ru, wu.at(i * TQ, on));
+            xn[R][i] = buf_load<T>(rx, wx.at(i * TQ, on));
+            if (GATED) zn[R][i] = buf_load<T>(rz, wz.at(i * TQ, on));
         }
     };
-    if (s0 < s1) fetch(s0);
-    for (int seg = s0; seg < s1; ++seg) {
-        float* buf = bc[seg & 1];
-        if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
-        __syncthreads();            // (the other buffer may still be read by a wave in the segment before)
+    const auto segment = [&](int seg, auto set) {
+        constexpr int R = decltype(set)::value;
         const int t0 = seg * SEG;
-        const bool full = t0 + SEG <= len;
+        float* buf = bc[R];
+        if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = raw_to_float(st[R], T{});
+        __syncthreads();            // (the other buffer may still be read by a wave in the segment before)
         float uc[Q], zc[Q], dt[Q], o[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            uc[i] = l.ocv ? (float)un[i] : 0.f;
-            const float x = l.ocv ? (float)xn[i] + bias : 0.f;
-            if (GATED) zc[i] = l.ocv ? (float)zn[i] : 0.f;
+            uc[i] = raw_to_float(un[R][i], T{});
+            const float x = raw_to_float(xn[R][i], T{}) + bias;
+            if (GATED) zc[i] = raw_to_float(zn[R][i], T{});
             dt[i] = p.softplus ? softplusf(x) : x;
-            if (!full) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;      // the state passes a padding frame
+            if (t0 + SEG > len) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;      // the state passes a padding frame
         }
-        if (seg + 1 < s1) fetch(seg + 1);
+        fetch(seg + 2, set);
         if (SAVE) {
             float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
@@ -380,22 +390,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             o[i] = quad_gather(acc, l.b0, l.b1) + Dv * uc[i];
             if (GATED) o[i] *= zc[i] * sigmoidf(zc[i]);
         }
-        if (l.ocv) {
-            if (full) {
+        const auto ry = wy.base(t0);
 #pragma unroll
-                for (int i = 0; i < Q; ++i) *wy.at(t0 + i * TQ) = (T)o[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < Q; ++i) {
-                    const int t = t0 + i * TQ + l.otp;
-                    if (t < p.T) *wy.at(t0 + i * TQ) = (T)(t < len ? o[i] : 0.f);
-                }
-            }
+        for (int i = 0; i < Q; ++i) {
+            const int t = t0 + i * TQ + l.otp;
+            buf_store<T>(ry, wy.at(i * TQ, t < p.T), t < len ? o[i] : 0.f);
+        }
+    };
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    if (s0 < s1) {
+        fetch(s0, even);
+        fetch(s0 + 1, odd);
+        for (int seg = s0; seg < s1; seg += 2) {
+            segment(seg, even);
+            if (seg + 1 < s1) segment(seg + 1, odd);
         }
     }
     const int end = min(p.T, (s0 + p.spc) * SEG);
     for (int t = max(nv, s0) * SEG; t < end; t += TQ)
-        if (l.ocv && t + l.otp < end) *wy.at(t) = (T)0.f;
+        if (l.ocv && t + l.otp < end) *wy.to(t) = (T)0.f;
     if (chunk == max(nv - 1, 0) / p.spc)
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -472,15 +486,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int turn = 0;
     float* flush_at = nullptr;                  // where the sums waiting in red[turn ^ 1] go
     auto flush = [&](const float (*rd)[SEG][16 * NS]) {
-        const int i = threadIdx.x, s = l.st_s, at = i % (8 * NS);
+        const int i = threadIdx.x, s = i / (8 * NS), at = i % (8 * NS);
         if (i < STAGE) flush_at[i] = ((rd[0][s][at] + rd[1][s][at]) + rd[2][s][at]) + rd[3][s][at];
     };
     const int b_end = min(p.B, (bg + 1) * p.per_bg);
     for (int b = bg * p.per_bg; b < b_end; ++b) {
         const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
-        const Walk<const T> wu(u, b, l.otp, l.ld), wx(delta, b, l.otp, l.ld), wz(z, b, l.otp, l.ld), wg(dy, b, l.otp, l.ld);
-        const Walk<T> wdu(du, b, l.otp, l.ld), wdx(ddelta, b, l.otp, l.ld), wdz(dz, b, l.otp, l.ld);
-        const Walk<const T> wb(l.st_which ? cm : bm, b, l.st_s, l.st_at);
+        const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv), wg(dy, b, l.otp, l.oc, l.ocv);
+        const Walk<T> wdu(du, b, l.otp, l.oc, l.ocv), wdx(ddelta, b, l.otp, l.oc, l.ocv), wdz(dz, b, l.otp, l.oc, l.ocv);
+        const Walk<const T> wb(bm, b, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
         float carry[NC][NS];
 #pragma unroll
         for (int k = 0; k < NC; ++k)
@@ -494,33 +508,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int c = (nv - 1) / p.spc; c > chunk; --c) carry_over<NS>(p, l, b, c, A2, carry);
         for (int t = max(nv, s0) * SEG; t < end; t += TQ)
             if (l.ocv && t + l.otp < end) {
-                *wdu.at(t) = (T)0.f;
-                *wdx.at(t) = (T)0.f;
-                if (GATED) *wdz.at(t) = (T)0.f;
+                *wdu.to(t) = (T)0.f;
+                *wdx.to(t) = (T)0.f;
+                if (GATED) *wdz.to(t) = (T)0.f;
             }
-        T un[Q], xn[Q], zn[Q], gn[Q], st;
+        uint32_t un[Q], xn[Q], zn[Q], gn[Q], st;
         float hn[P];
-        auto fetch = [&](int seg) {
-            const int t0 = seg * SEG;
-            if (t0 + SEG <= len) {
-                st = *wb.at(t0);
+        const auto fetch = [&](int of) {                // before the first segment: the first one again
+            const int seg = max(of, s0), t0 = seg * SEG;
+            const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0), rg = wg.base(t0);
+            st = buf_load<T>(wb.base(t0), wb.at(0, l.st_s < len - t0)) | buf_load<T>(wc.base(t0), wc.at(0, l.st_s < len - t0));
 #pragma unroll
-                for (int i = 0; i < Q; ++i) {
-                    un[i] = *wu.at(t0 + i * TQ);
-                    xn[i] = *wx.at(t0 + i * TQ);
-                    gn[i] = *wg.at(t0 + i * TQ);
-                    if (GATED) zn[i] = *wz.at(t0 + i * TQ);
-                }
-            } else {
-                st = t0 + l.st_s < len ? *wb.at(t0) : (T)0.f;
-#pragma unroll
-                for (int i = 0; i < Q; ++i) {
-                    const bool on = t0 + i * TQ + l.otp < len;
-                    un[i] = on ? *wu.at(t0 + i * TQ) : (T)0.f;
-                    xn[i] = on ? *wx.at(t0 + i * TQ) : (T)0.f;
-                    gn[i] = on ? *wg.at(t0 + i * TQ) : (T)0.f;
-                    if (GATED) zn[i] = on ? *wz.at(t0 + i * TQ) : (T)0.f;
-                }
+            for (int i = 0; i < Q; ++i) {
+                const bool on = t0 + i * TQ + l.otp < len;
+                un[i] = buf_load<T>(ru, wu.at(i * TQ, on));
+                xn[i] = buf_load<T>(rx, wx.at(i * TQ, on));
+                gn[i] = buf_load<T>(rg, wg.at(i * TQ, on));
+                if (GATED) zn[i] = buf_load<T>(rz, wz.at(i * TQ, on));
             }
             const float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
@@ -529,7 +533,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (s0 < s1) fetch(s1 - 1);
         for (int seg = s1 - 1; seg >= s0; --seg) {
             float* buf = bc[turn];
-            if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = l.st_on ? (float)st : 0.f;
+            if ((int)threadIdx.x < STAGE) buf[threadIdx.x] = raw_to_float(st, T{});
             __syncthreads();                    // B and C are in; the sums of the segment before are complete
             if (flush_at) flush(red[turn ^ 1]);
             flush_at = p.part_bc + ((((int64_t)(cblk - l.g * p.bpg) * p.B + b) * p.nseg + seg) * p.G + l.g) * STAGE;
@@ -538,16 +542,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             float uc[Q], xc[Q], zc[Q], gc[Q], dt[Q], h[NC][NS], odu[Q], odx[Q], odz[Q];
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
-                uc[i] = l.ocv ? (float)un[i] : 0.f;
-                xc[i] = l.ocv ? (float)xn[i] + bias : 0.f;
-                gc[i] = l.ocv ? (float)gn[i] : 0.f;
-                if (GATED) zc[i] = l.ocv ? (float)zn[i] : 0.f;
+                uc[i] = raw_to_float(un[i], T{});
+                xc[i] = raw_to_float(xn[i], T{}) + bias;
+                gc[i] = raw_to_float(gn[i], T{});
+                if (GATED) zc[i] = raw_to_float(zn[i], T{});
                 dt[i] = p.softplus ? softplusf(xc[i]) : xc[i];
                 if (!full) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;
             }
 #pragma unroll
             for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
-            if (seg > s0) fetch(seg - 1);
+            fetch(seg - 1);
             float a[SEG][NC][NS], e[SEG][NC][NS], bn[NS], cn[NS];
             load_vec<float, NS>(buf + l.ng * NS, bn);
 #pragma unroll
@@ -621,14 +625,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 dD += dyp * uc[i];
                 if (GATED) odz[i] = gc[i] * (quad_gather(sy, l.b0, l.b1) + Dv * uc[i]) * sg * (1.f + zc[i] * (1.f - sg));
             }
-            if (l.ocv) {
+            const auto rdu = wdu.base(t0), rdx = wdx.base(t0), rdz = wdz.base(t0);
 #pragma unroll
-                for (int i = 0; i < Q; ++i)
-                    if (full || t0 + i * TQ + l.otp < p.T) {
-                        *wdu.at(t0 + i * TQ) = (T)odu[i];
-                        *wdx.at(t0 + i * TQ) = (T)odx[i];
-                        if (GATED) *wdz.at(t0 + i * TQ) = (T)odz[i];
-                    }
+            for (int i = 0; i < Q; ++i) {
+                const bool on = t0 + i * TQ + l.otp < p.T;
+                buf_store<T>(rdu, wdu.at(i * TQ, on), odu[i]);
+                buf_store<T>(rdx, wdx.at(i * TQ, on), odx[i]);
+                if (GATED) buf_store<T>(rdz, wdz.at(i * TQ, on), odz[i]);
             }
             turn ^= 1;
         }
@@ -821,10 +824,10 @@ int check(const adn_scan_args* a, const char* who, bool backward) {
     ADN_CHECK(sizes_ok(a->batch, a->steps, a->channels, a->states, a->groups), ADN_ERR_INVALID, std::string(who) + ": batch * channels too large");
     ADN_CHECK(a->A, ADN_ERR_INVALID, std::string(who) + ": null A");
     const int e = a->dtype == ADN_DTYPE_BF16 ? 2 : 4;
-    // 32-bit offsets within a segment: three frames on, and a channel
-    const auto far = [](const adn_seq& t) { return t.data && (t.stride_t < 0 || t.stride_t >= (int64_t)1 << 28); };
+    // 31-bit offsets within a segment: seven frames on, and a channel
+    const auto far = [](const adn_seq& t) { return t.data && (t.stride_t < 0 || t.stride_t >= (int64_t)1 << 26); };
     ADN_CHECK(!far(a->u) && !far(a->delta) && !far(a->b) && !far(a->c) && !far(a->z) && !far(a->y) && !far(a->dy) && !far(a->du) && !far(a->ddelta) && !far(a->dz),
-              ADN_ERR_INVALID, std::string(who) + ": a frame stride outside 0 .. 2^28");
+              ADN_ERR_INVALID, std::string(who) + ": a frame stride outside 0 .. 2^26");
     if ((int64_t)a->batch * a->steps > 0) {
         ADN_CHECK(seq_ok(a->u, e) && seq_ok(a->delta, e) && seq_ok(a->b, e) && seq_ok(a->c, e), ADN_ERR_INVALID, std::string(who) + ": null or misaligned tensor");
         ADN_CHECK(!a->z.data || seq_ok(a->z, e), ADN_ERR_INVALID, std::string(who) + ": misaligned gate");
