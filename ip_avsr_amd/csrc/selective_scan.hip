@@ -126,19 +126,21 @@ static_assert(Place<1>::SPT == 1 && Place<2>::SPT == 1 && Place<4>::SPT == 1 && 
 // check turns away: its load is 0, its store is dropped, and no branch stands between the loads in flight
 constexpr uint32_t kNowhere = 0x80000000u;
 template <typename T> struct Walk {
-    const char* p;
+    char* p;                           // the segment's first frame
     uint32_t frame;                    // bytes between frames
     uint32_t off;                      // of the lane's first frame in a segment
-    __device__ __forceinline__ Walk(const View<T>& v, int b, int frame_of_lane, int c, bool on)
-        : p(reinterpret_cast<const char*>(v.p + b * v.sb)), frame((uint32_t)v.st * (uint32_t)sizeof(T)),
+    __device__ __forceinline__ Walk(const View<T>& v, int b, int t0, int frame_of_lane, int c, bool on)
+        : p(reinterpret_cast<char*>(const_cast<std::remove_const_t<T>*>(v.p + b * v.sb + t0 * v.st))), frame((uint32_t)v.st * (uint32_t)sizeof(T)),
           off(on ? (uint32_t)frame_of_lane * frame + (uint32_t)c * (uint32_t)sizeof(T) : kNowhere) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t base() const { return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7FFFFFFF, 0x00027000); }
+    // ... where the walk stays at its start: the backward pass holds seven of them and has no scalar registers to move them in
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t base(int t0) const {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame), 0, 0x7FFFFFFF, 0x00027000);
+        return __builtin_amdgcn_make_buffer_rsrc(p + (uint64_t)(uint32_t)t0 * frame, 0, 0x7FFFFFFF, 0x00027000);
     }
+    // on by FRAMES; a place outside the tensor is harmless as long as every lane is turned away there
+    template <int FRAMES> __device__ __forceinline__ void move() { p += (int64_t)FRAMES * (int64_t)frame; }
     // `ahead` frames behind the lane's first; `on`: whether there is such a frame
     __device__ __forceinline__ uint32_t at(int ahead, bool on) const { return on ? off + (uint32_t)ahead * frame : kNowhere; }
-    // without bounds, for the frames behind the last segment
-    __device__ __forceinline__ T* to(int t0) const { return reinterpret_cast<T*>(const_cast<char*>(p + (uint64_t)(uint32_t)t0 * frame) + off); }
 };
 __device__ __forceinline__ float raw_to_float(uint32_t v, float) { return __builtin_bit_cast(float, v); }
 __device__ __forceinline__ float raw_to_float(uint32_t v, __bf16) { return __builtin_bit_cast(float, v << 16); }
@@ -205,23 +207,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             h[k][j] = !BACK && on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
     const float bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
-    const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv);
+    const int first = (BACK ? s1 - 1 : s0) * SEG;
+    Walk<const T> wu(u, b, first, l.otp, l.oc, l.ocv), wx(delta, b, first, l.otp, l.oc, l.ocv), wz(z, b, BACK && GATED ? first : 0, l.otp, l.oc, l.ocv);
     const int ms = (int)threadIdx.x / (4 * NS), mn = (int)threadIdx.x % (4 * NS);
     const bool mon = (int)threadIdx.x < ROWS && mn < p.N;
-    const Walk<const T> wm(m, b, ms, l.g * p.N + mn, mon);
+    Walk<const T> wm(m, b, first, ms, l.g * p.N + mn, mon);
     uint32_t un[2][Q], xn[2][Q], zn[2][Q], st[2];
-    const auto fetch = [&](int k0, auto set) {          // the k0-th segment of the piece; none: the last one again
+    int ft = first;
+    const auto fetch = [&](auto set) {                  // the next segment on the way; outside the utterance nothing
         constexpr int R = decltype(set)::value;
-        const int k = min(k0, s1 - s0 - 1), t0 = (BACK ? s1 - 1 - k : s0 + k) * SEG;
-        const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0);
-        st[R] = buf_load<T>(wm.base(t0), wm.at(0, ms < len - t0));
+        const auto ru = wu.base(), rx = wx.base(), rz = wz.base();
+        st[R] = buf_load<T>(wm.base(), wm.at(0, (unsigned)(ft + ms) < (unsigned)len));
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            const bool on = t0 + i * TQ + l.otp < len;
+            const bool on = (unsigned)(ft + i * TQ + l.otp) < (unsigned)len;
             un[R][i] = buf_load<T>(ru, wu.at(i * TQ, on));
             xn[R][i] = buf_load<T>(rx, wx.at(i * TQ, on));
             if (BACK && GATED) zn[R][i] = buf_load<T>(rz, wz.at(i * TQ, on));
         }
+        constexpr int ON = BACK ? -SEG : SEG;
+        ft += ON;
+        wu.template move<ON>();
+        wx.template move<ON>();
+        wm.template move<ON>();
+        if (BACK && GATED) wz.template move<ON>();
     };
     float total = 0.f;
     const int n = s1 - s0;
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             else if (GATED) { const float zc = raw_to_float(zn[R][i], T{}); in[i] *= zc * sigmoidf(zc); }
             total += dt[i];
         }
-        fetch(k0 + 2, set);
+        fetch(set);
         float mn1[NS];
         load_vec<float, NS>(buf + (BACK ? SEG - 1 : 0) * 4 * NS + l.ng * NS, mn1);
 #pragma unroll
@@ -270,8 +279,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    fetch(0, even);
-    fetch(1, odd);
+    fetch(even);
+    fetch(odd);
     for (int k0 = 0; k0 < n; k0 += 2) {
         segment(k0, even);
         if (k0 + 1 < n) segment(k0 + 1, odd);
@@ -313,23 +322,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     if (s0 < nv)
         for (int c = 0; c < chunk; ++c) carry_over<NS>(p, l, b, c, A2, h);
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
-    const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv);
-    const Walk<T> wy(y, b, l.otp, l.oc, l.ocv);
-    const Walk<const T> wb(bm, b, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
+    int ft = s0 * SEG;
+    Walk<const T> wu(u, b, ft, l.otp, l.oc, l.ocv), wx(delta, b, ft, l.otp, l.oc, l.ocv), wz(z, b, GATED ? ft : 0, l.otp, l.oc, l.ocv);
+    Walk<T> wy(y, b, ft, l.otp, l.oc, l.ocv);
+    Walk<const T> wb(bm, b, ft, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, ft, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
     // a segment's loads are issued two segments ahead, into one of two sets of registers
     uint32_t un[2][Q], xn[2][Q], zn[2][Q], st[2];
-    const auto fetch = [&](int of, auto set) {          // behind the last segment: the last one again
+    const auto fetch = [&](auto set) {                  // the next segment; behind the utterance nothing
         constexpr int R = decltype(set)::value;
-        const int t0 = min(of, s1 - 1) * SEG;
-        const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0);
-        st[R] = buf_load<T>(wb.base(t0), wb.at(0, l.st_s < len - t0)) | buf_load<T>(wc.base(t0), wc.at(0, l.st_s < len - t0));
+        const auto ru = wu.base(), rx = wx.base(), rz = wz.base();
+        const bool rows = l.st_s < len - ft;
+        st[R] = buf_load<T>(wb.base(), wb.at(0, rows)) | buf_load<T>(wc.base(), wc.at(0, rows));
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-            const bool on = t0 + i * TQ + l.otp < len;
+            const bool on = ft + i * TQ + l.otp < len;
             un[R][i] = buf_load<T>(ru, wu.at(i * TQ, on));
             xn[R][i] = buf_load<T>(rx, wx.at(i * TQ, on));
             if (GATED) zn[R][i] = buf_load<T>(rz, wz.at(i * TQ, on));
         }
+        ft += SEG;
+        wu.template move<SEG>();
+        wx.template move<SEG>();
+        wb.template move<SEG>();
+        wc.template move<SEG>();
+        if (GATED) wz.template move<SEG>();
     };
     const auto segment = [&](int seg, auto set) {
         constexpr int R = decltype(set)::value;
@@ -346,7 +362,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             dt[i] = p.softplus ? softplusf(x) : x;
             if (t0 + SEG > len) dt[i] = t0 + i * TQ + l.otp < len ? dt[i] : 0.f;      // the state passes a padding frame
         }
-        fetch(seg + 2, set);
+        fetch(set);
         if (SAVE) {
             float* ck = p.ckpt + ckpt_at<P>(p, b, seg, l.ctile) + l.lane * 4;
 #pragma unroll
@@ -390,26 +406,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             o[i] = quad_gather(acc, l.b0, l.b1) + Dv * uc[i];
             if (GATED) o[i] *= zc[i] * sigmoidf(zc[i]);
         }
-        const auto ry = wy.base(t0);
+        const auto ry = wy.base();
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
             const int t = t0 + i * TQ + l.otp;
             buf_store<T>(ry, wy.at(i * TQ, t < p.T), t < len ? o[i] : 0.f);
         }
+        wy.template move<SEG>();
     };
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
     if (s0 < s1) {
-        fetch(s0, even);
-        fetch(s0 + 1, odd);
+        fetch(even);
+        fetch(odd);
         for (int seg = s0; seg < s1; seg += 2) {
             segment(seg, even);
             if (seg + 1 < s1) segment(seg + 1, odd);
         }
     }
     const int end = min(p.T, (s0 + p.spc) * SEG);
-    for (int t = max(nv, s0) * SEG; t < end; t += TQ)
-        if (l.ocv && t + l.otp < end) *wy.to(t) = (T)0.f;
+    for (int t = max(nv, s0) * SEG + l.otp; t < end; t += TQ)
+        if (l.ocv) y.row(b, t)[l.oc] = (T)0.f;
     if (chunk == max(nv - 1, 0) / p.spc)
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -492,9 +509,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int b_end = min(p.B, (bg + 1) * p.per_bg);
     for (int b = bg * p.per_bg; b < b_end; ++b) {
         const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
-        const Walk<const T> wu(u, b, l.otp, l.oc, l.ocv), wx(delta, b, l.otp, l.oc, l.ocv), wz(z, b, l.otp, l.oc, l.ocv), wg(dy, b, l.otp, l.oc, l.ocv);
-        const Walk<T> wdu(du, b, l.otp, l.oc, l.ocv), wdx(ddelta, b, l.otp, l.oc, l.ocv), wdz(dz, b, l.otp, l.oc, l.ocv);
-        const Walk<const T> wb(bm, b, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
         float carry[NC][NS];
 #pragma unroll
         for (int k = 0; k < NC; ++k)
@@ -506,18 +520,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc), end = min(p.T, (s0 + p.spc) * SEG);
         if (s0 < nv)
             for (int c = (nv - 1) / p.spc; c > chunk; --c) carry_over<NS>(p, l, b, c, A2, carry);
-        for (int t = max(nv, s0) * SEG; t < end; t += TQ)
-            if (l.ocv && t + l.otp < end) {
-                *wdu.to(t) = (T)0.f;
-                *wdx.to(t) = (T)0.f;
-                if (GATED) *wdz.to(t) = (T)0.f;
+        for (int t = max(nv, s0) * SEG + l.otp; t < end; t += TQ)
+            if (l.ocv) {
+                du.row(b, t)[l.oc] = (T)0.f;
+                ddelta.row(b, t)[l.oc] = (T)0.f;
+                if (GATED) dz.row(b, t)[l.oc] = (T)0.f;
             }
+        const Walk<const T> wu(u, b, 0, l.otp, l.oc, l.ocv), wx(delta, b, 0, l.otp, l.oc, l.ocv), wz(z, b, 0, l.otp, l.oc, l.ocv), wg(dy, b, 0, l.otp, l.oc, l.ocv);
+        const Walk<T> wdu(du, b, 0, l.otp, l.oc, l.ocv), wdx(ddelta, b, 0, l.otp, l.oc, l.ocv), wdz(dz, b, 0, l.otp, l.oc, l.ocv);
+        const Walk<const T> wb(bm, b, 0, l.st_s, l.st_at, l.st_s < SEG && !l.st_which), wc(cm, b, 0, l.st_s, l.st_at, l.st_s < SEG && l.st_which);
         uint32_t un[Q], xn[Q], zn[Q], gn[Q], st;
         float hn[P];
         const auto fetch = [&](int of) {                // before the first segment: the first one again
             const int seg = max(of, s0), t0 = seg * SEG;
             const auto ru = wu.base(t0), rx = wx.base(t0), rz = wz.base(t0), rg = wg.base(t0);
-            st = buf_load<T>(wb.base(t0), wb.at(0, l.st_s < len - t0)) | buf_load<T>(wc.base(t0), wc.at(0, l.st_s < len - t0));
+            const bool rows = l.st_s < len - t0;
+            st = buf_load<T>(wb.base(t0), wb.at(0, rows)) | buf_load<T>(wc.base(t0), wc.at(0, rows));
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
                 const bool on = t0 + i * TQ + l.otp < len;
