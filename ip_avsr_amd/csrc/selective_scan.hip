@@ -820,6 +820,10 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G, bool bwd) {
         q.chunks = (int)std::min<int64_t>(q.nseg / kMinPiece, (4096 + waves - 1) / waves);
     q.spc = std::max(1, cdiv(q.nseg, q.chunks));
     q.chunks = std::max(1, cdiv(q.nseg, q.spc));
+    if (q.chunks > 1) {      // the pieces' launches go by utterance (so few waves make groups of one anyway)
+        q.per_bg = 1;
+        q.nbg = (int)B;
+    }
     q.local = q.chunks > 1 ? B * q.chunks * q.ctiles * 64 * P : 0;
     q.dsum = q.chunks > 1 ? B * q.chunks * q.ctiles * WC : 0;
     q.part_bc = (int64_t)q.bpg * B * q.nseg * G * seg * 8 * q.ns;
@@ -843,7 +847,7 @@ int check(const adn_scan_args* a, const char* who, bool backward) {
     ADN_CHECK(a->A, ADN_ERR_INVALID, std::string(who) + ": null A");
     const int e = a->dtype == ADN_DTYPE_BF16 ? 2 : 4;
     // 31-bit offsets within a segment: seven frames on, and a channel
-    const auto far = [](const adn_seq& t) { return t.data && (t.stride_t < 0 || t.stride_t >= (int64_t)1 << 26); };
+    const auto far = [&](const adn_seq& t) { return a->steps > 1 && t.data && (t.stride_t < 0 || t.stride_t >= (int64_t)1 << 26); };
     ADN_CHECK(!far(a->u) && !far(a->delta) && !far(a->b) && !far(a->c) && !far(a->z) && !far(a->y) && !far(a->dy) && !far(a->du) && !far(a->ddelta) && !far(a->dz),
               ADN_ERR_INVALID, std::string(who) + ": a frame stride outside 0 .. 2^26");
     if ((int64_t)a->batch * a->steps > 0) {

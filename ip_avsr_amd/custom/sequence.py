@@ -11,7 +11,8 @@ call in the same type, with dense channels and any frame and utterance stride (c
 arrays); parameters, statistics and the scan's states in float32, dense.  Results are new dense tensors.  ``lens`` (int32, one length
 per utterance) marks frames at and behind it as padding: never read, zero in every result, absent from every sum, and a state passes
 them unchanged; lengths outside [0, T] are clamped.  Work is enqueued on the current stream of the tensors' device; sums run in a
-fixed order, so two runs give the same bits.  A bad argument raises ``ValueError``; without the HIP library the first call raises.
+fixed order, so two runs give the same bits.  A bad argument raises ``ValueError``, sizes that the library refuses ``AdenetError``;
+without the HIP library the first call raises.
 """
 import ctypes as C
 

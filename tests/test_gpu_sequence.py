@@ -494,3 +494,88 @@ def test_captured_into_graphs(S):
             torch.cuda.synchronize()
             for got, want in zip(outs[k], eager[k]):
                 assert torch.equal(got, want)
+
+
+def test_frames_more_than_4_gib_apart(S):
+    """Rows 8 MiB apart, 700 of them: the same bits as from a dense copy."""
+    torch = _torch()
+    T, D, wide = 700, 64, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")                   # noqa: E731
+    big = torch.empty(1, T, wide, dtype=torch.bfloat16, device="cuda")           # 5.5 GiB; only the columns below are written or read
+    cols = [big[..., k * 128:k * 128 + D] for k in range(4)]
+    dense = [rn(1, T, D).bfloat16() for _ in cols]
+    for c, d in zip(cols, dense):
+        c.copy_(d)
+    gamma, beta, w = rn(D), rn(D), rn(4, D)
+    A, bm = -torch.rand(D, 16, generator=g, device="cuda"), rn(1, T, 16).bfloat16()
+    rows = big[..., 1 << 20:(1 << 20) + 16]
+    rows.copy_(bm)
+
+    def passes(x, u, z, dy, bm):
+        y, m, i = S.layer_norm_forward(x, gamma, beta)
+        out = [y, m, i] + list(S.layer_norm_backward(dy, x, gamma, m, i))
+        y, st = S.causal_conv_forward(x, w, beta)
+        out += [y, st] + list(S.causal_conv_backward(dy, x, w, beta)[:3])
+        y, st, saved = S.selective_scan_forward(u, x, A, bm, bm, D=gamma, z=z, save=True)
+        grads = S.selective_scan_backward(dy, u, x, A, bm, bm, saved, D=gamma, z=z)
+        return out + [y, st] + [v for v in grads.values() if v is not None]
+    for a, b in zip(passes(*cols, rows), passes(*dense, bm)):
+        assert torch.equal(a, b)
+
+
+def test_many_utterances(S):
+    """More utterances than a grid dimension holds."""
+    torch = _torch()
+    B, D, N = 70001, 6, 3
+    g = torch.Generator(device="cuda").manual_seed(12)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")                   # noqa: E731
+    x, st, w = rn(B, D), rn(B, 2, D), rn(3, D)
+    want = (torch.cat([st, x[:, None]], 1) * w).sum(1)
+    after = torch.cat([st[:, 1:], x[:, None]], 1)
+    y = S.causal_conv_step(x, st, w, activation="linear")
+    # three products and their sum: 5 roundings of at most the sum of the sizes
+    size = (torch.cat([st, x[:, None]], 1).abs().amax(1) * w.abs().sum(0)).max() + x.abs().max() * w.abs().sum(0).max()
+    assert (y - want).abs().max() <= 5 * 2.0 ** -24 * 4 * size and torch.equal(st, after)
+    A, bc, h = -torch.rand(D, N, generator=g, device="cuda"), rn(B, N), rn(B, D, N)
+    dt = torch.rand(B, D, generator=g, device="cuda")
+    want_h = torch.exp(dt.double()[..., None] * A.double()) * h.double() + (dt.double() * x.double())[..., None] * bc.double()[:, None]
+    y = S.selective_scan_step(x, dt, A, bc, bc, h, softplus=False)
+    # h: a and its product, dt u B: about 12 roundings of the sizes (all below 40)
+    assert (h - want_h).abs().max() <= 12 * 2.0 ** -24 * 40
+    assert (y - (want_h * bc.double()[:, None]).sum(-1)).abs().max() <= 20 * 2.0 ** -24 * 40 * 5 * N
+    u = rn(B, 2, D)
+    y, last, _ = S.selective_scan_forward(u, dt[:, None].expand(B, 2, D), A, bc[:, None].expand(B, 2, N), bc[:, None].expand(B, 2, N), softplus=False)
+    h = torch.zeros(B, D, N, device="cuda")
+    for t in range(2):
+        yt = S.selective_scan_step(u[:, t], dt, A, bc, bc, h, softplus=False)
+        assert (y[:, t] - yt).abs().max() <= 20 * 2.0 ** -24 * 40 * 5 * N
+    assert (last - h).abs().max() <= 24 * 2.0 ** -24 * 40
+
+
+def test_two_streams_at_once(S):
+    torch = _torch()
+    sets = [_block_inputs(4, 150, 24, 72, 16, seed=k) for k in (21, 22)]
+    want = [_block(S, t, w, None) for t, w in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [None, None]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k] = _block(S, *sets[k], None)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for k in a:
+            assert torch.equal(a[k], b[k]), k
+
+
+def test_sizes_that_the_library_refuses(S):
+    torch = _torch()
+    from ip_avsr_amd._lib import AdenetError
+    x = torch.zeros(1, 1, 16385, device="cuda")
+    with pytest.raises(AdenetError, match="channels"):
+        S.layer_norm_forward(x)
+    with pytest.raises(ValueError, match="out of range"):
+        S.layer_norm_backward(x, x, None, torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, device="cuda"))
+    with pytest.raises(AdenetError, match="eps"):
+        S.layer_norm_forward(x[..., :8].contiguous(), eps=-1.0)

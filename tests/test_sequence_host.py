@@ -95,7 +95,7 @@ def test_causal_conv_backward_and_step_refusals(lib):
 @pytest.mark.parametrize("over,word", [
     (dict(dtype=3), "dtype"), (dict(states=0), "states"), (dict(states=33), "states"), (dict(groups=3), "groups"), (dict(groups=0), "groups"),
     (dict(A=None), "A"), (dict(u=None), "tensor"), (dict(z=2), "gate"), (dict(y=None), "y"), (dict(state_out=None), "state_out"),
-    (dict(state=64), "state_out"), (dict(batch=1 << 20, steps=1, channels=1 << 12), "too large"), (dict(checkpoints=64, checkpoint_floats=1), "checkpoints")])
+    (dict(state=64), "state_out"), (dict(u_stride_t=1 << 26), "frame stride"), (dict(c_stride_t=-8), "frame stride"), (dict(batch=1 << 20, steps=1, channels=1 << 12), "too large"), (dict(checkpoints=64, checkpoint_floats=1), "checkpoints")])
 def test_selective_scan_refusals(lib, over, word):
     _refused(lib.adn_op_selective_scan_forward, _scan(**over), word, lib)
 
