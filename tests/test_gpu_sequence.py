@@ -579,3 +579,51 @@ def test_sizes_that_the_library_refuses(S):
         S.layer_norm_backward(x, x, None, torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, device="cuda"))
     with pytest.raises(AdenetError, match="eps"):
         S.layer_norm_forward(x[..., :8].contiguous(), eps=-1.0)
+
+
+def _random_lens(d, B, T):
+    return [int(v) for v in d.rng.integers(0, T + 1, size=B)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(110, 60, 40), (30, 40, 1100), (26, 40, 2056), (3, 100, 4104), (3, 100, 8200), (2, 150, 4001), (2, 150, 9001)],
+                         ids=lambda v: "x".join(map(str, v)))
+def test_layer_norm_over_many_rows(S, dtype, shape):
+    """More rows than workgroups, in every width of a row: the workgroups' own sums and their sum over workgroups."""
+    d = Draw(("norm rows", shape), dtype)
+    lens = _random_lens(d, shape[0], shape[1])
+    (xv, x), (gv, g), (dyv, dy) = d.seq(*shape, lens=lens), d.param(shape[2], scale=0.3, shift=1), d.seq(*shape, lens=lens)
+    want = O.layer_norm(xv, gv, None, 1e-5, lens, dyv)
+    y, mean, inv = S.layer_norm_forward(x, g, lens=_lens(lens))
+    dx, dg, db = S.layer_norm_backward(dy, x, g, mean, inv, lens=_lens(lens))
+    for name, got, t in (("y", y, dtype), ("mean", mean, "float32"), ("inv_std", inv, "float32"), ("dx", dx, dtype), ("dgamma", dg, "float32"), ("dbeta", db, "float32")):
+        _near(name, got, want[name], t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_short_utterances(S, dtype):
+    """More utterances than workgroups: several per workgroup, their sums in its registers."""
+    d = Draw("short", dtype)
+    lens = _random_lens(d, 5000, 3)
+    (xv, x), (wv, w), (dyv, dy) = d.seq(5000, 3, 8, lens=lens), d.param(3, 8), d.seq(5000, 3, 8, lens=lens)
+    want = O.causal_conv(xv, wv, None, None, lens, "silu", dyv)
+    y, st = S.causal_conv_forward(x, w, lens=_lens(lens))
+    dx, dw, db, _ = S.causal_conv_backward(dy, x, w, lens=_lens(lens))
+    _near("y", y, want["y"], dtype)
+    _near("dx", dx, want["dx"], dtype)
+    _near("dweight", dw, want["dweight"])
+    _near("dbias", db, want["dbias"])
+    np.testing.assert_array_equal(st.double().cpu().numpy(), want["state"].v)
+    B, T, D, N = 2500, 3, 20, 4
+    lens = _random_lens(d, B, T)
+    v, t = _scan_inputs(d, (B, T, D), N, 1, lens, True, True, True)
+    dyv, dy = d.seq(B, T, D, lens=lens)
+    want = O.selective_scan(dy=dyv, **v)
+    y, state, saved = S.selective_scan_forward(save=True, **t)
+    got = S.selective_scan_backward(dy, saved=saved, **t)
+    _near("y", y, want["y"], dtype)
+    _near("state", state, want["state"])
+    for name in ("du", "ddelta", "dB", "dC", "dz"):
+        _near(name, got[name], want[name], dtype)
+    for name in ("dA", "dD", "ddelta_bias", "dstate"):
+        _near(name, got[name], want[name])
