@@ -16,7 +16,7 @@
 // reduction of 4 values over the quad (9 instructions) that leaves each lane the one it owns.  A workgroup is 4 waves of 16 NC
 // channels.  More states per lane would save a tenth of the instructions and cost the registers that the backward pass needs.
 //
-// Frames go by segments of 8 (4 where N > 16), the loads of the next one in flight; a whole segment has no branch in it.  The backward
+// Frames go by segments of 8 (4 where N > 16 or N <= 4), the loads of the next ones in flight; a segment has no branch in it.  The backward
 // pass walks them from the end: from the state the forward pass kept at the segment's start it recomputes a and e of the segment into
 // registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by exchanging halves (permlane swaps, row
 // rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
@@ -54,10 +54,11 @@ struct ScanParams {
     int softplus;
 };
 
-// channels of a quad and frames of a segment: 4 (channel, state) pairs per lane and 8 frames, 8 and 4 where N > 16 -- what a and e of
-// a segment take in registers is the same
+// channels of a quad and frames of a segment: 4 (channel, state) pairs per lane and 8 frames; 8 pairs and 4 frames where N > 16, which
+// keeps what a segment takes in registers, and 4 frames where N <= 4, whose lanes own a frame of every channel and would spill the rest
+// (32 x 512 x 2048 x 4: backward 228 us, with 8 frames 273; of 8 states 8 frames 303 us, 4 frames 344)
 constexpr int channels_per_quad(int ns) { return ns == 8 ? 1 : 4 / ns; }
-constexpr int segment_frames(int ns) { return ns == 8 ? 4 : 8; }
+constexpr int segment_frames(int ns) { return ns == 1 || ns == 8 ? 4 : 8; }
 
 // log(1 + exp(x)), relative accuracy also where it is small: log1p(e) = 2 atanh(e / (2 + e)) of e = exp(-|x|) <= 1, whose odd series
 // in s = e / (2 + e) <= 1/3 is cut where the rest is below 2^-26 of it
@@ -483,6 +484,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                                                                View<const T> dy, View<T> du, View<T> ddelta, View<T> dz, ScanParams p) {
     using L = Place<NS>;
     constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, WC = L::WC, SEG = L::SEG, STAGE = L::STAGE;
+    constexpr bool KEEP = NS >= 4;                      // the segment's states too, not a and e alone: a multiply-add less, where registers are left
     __shared__ __align__(16) float bc[2][STAGE];
     __shared__ float red[2][4][SEG][16 * NS];           // per frame 8 NS sums and 8 NS places nobody reads
     const int cb = p.bpg * p.G;
@@ -570,7 +572,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int m = 0; m < P; ++m) h[m / NS][m % NS] = hn[m];
             fetch(seg - 1);
-            float a[SEG][NC][NS], e[SEG][NC][NS], bn[NS], cn[NS];
+            float a[SEG][NC][NS], e[SEG][NC][NS], hs[KEEP ? SEG : 1][NC][NS], bn[NS], cn[NS];
             load_vec<float, NS>(buf + l.ng * NS, bn);
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
@@ -592,6 +594,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                             a[s][k][j] = __builtin_amdgcn_exp2f(dtk * A2[k][j]);
                             e[s][k][j] = a[s][k][j] * h[k][j];
                             h[k][j] = fmaf(dtuk, bv[j], e[s][k][j]);
+                            if (KEEP) hs[s][k][j] = h[k][j];
                         }
                     }
                 }
@@ -621,7 +624,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         const float dtk = bcast(dt[i], q), dtuk = bcast(dtu, q), dyk = bcast(dyp, q);
 #pragma unroll
                         for (int j = 0; j < NS; ++j) {
-                            const float dh = fmaf(cv[j], dyk, carry[k][j]), hv = fmaf(dtuk, bv[j], e[s][k][j]), de = dh * e[s][k][j];
+                            const float dh = fmaf(cv[j], dyk, carry[k][j]), hv = KEEP ? hs[s][k][j] : fmaf(dtuk, bv[j], e[s][k][j]), de = dh * e[s][k][j];
                             sums[j] = fmaf(dtuk, dh, sums[j]);
                             sums[NS + j] = fmaf(dyk, hv, sums[NS + j]);
                             s1[q] = fmaf(dh, bv[j], s1[q]);
