@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                                                                View<const T> dy, View<T> du, View<T> ddelta, View<T> dz, ScanParams p) {
     using L = Place<NS>;
     constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, WC = L::WC, SEG = L::SEG, STAGE = L::STAGE;
-    constexpr bool KEEP = NS >= 4;                      // the segment's states too, not a and e alone: a multiply-add less, where registers are left
+    constexpr bool KEEP = NS != 2;                      // the segment's states too, not a and e alone: a multiply-add less, where registers are left
     __shared__ __align__(16) float bc[2][STAGE];
     __shared__ float red[2][4][SEG][16 * NS];           // per frame 8 NS sums and 8 NS places nobody reads
     const int cb = p.bpg * p.G;
