@@ -21,6 +21,9 @@
 // registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by exchanging halves (permlane swaps, row
 // rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
 // over all frames of a workgroup's utterances.  All sums run in a fixed order.
+// 8 x 2048 x 2048 x 16 bfloat16, gated: forward 280 us with what training keeps, 0.52 us per 10^6 (t, d, n) where the 8 slots take 0.20
+// (1024 waves, one per SIMD: the issue of that one is the limit; with four per SIMD 0.33), backward 468 us (27 vector instructions a
+// (t, d, n), the pipe 83 % busy) behind 121 us for the pieces alone.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
 #include <type_traits>
