@@ -346,7 +346,7 @@ extern "C" int adn_op_causal_conv_forward(const adn_conv_args* a, void* hip_stre
                     ptr_aligned(a->state, 16) && ptr_aligned(a->state_out, 16);
     p.run = run_length(p.B, std::max(p.T, 1), cdiv(p.C, 64 * (al ? v : 1)));
     p.runs = std::max(1, cdiv(p.T, p.run));      // (no frames: the history is still handed on)
-    ADN_CHECK((int64_t)p.B * p.runs < ((int64_t)1 << 31) - 65536, ADN_ERR_INVALID, "adn_op_causal_conv_forward: batch too large");
+    ADN_CHECK(grid_ok(((int64_t)p.B * p.runs + 3) / 4), ADN_ERR_INVALID, "adn_op_causal_conv_forward: batch too large");
     if (a->dtype == ADN_DTYPE_BF16) return al ? launch<__bf16, 8, kForward>(*a, p, s) : launch<__bf16, 1, kForward>(*a, p, s);
     return al ? launch<float, 4, kForward>(*a, p, s) : launch<float, 1, kForward>(*a, p, s);
 }

@@ -913,7 +913,6 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
 #undef ADN_SCAN_GO
     const int64_t bc = (int64_t)p.B * p.T * p.G * p.N * 2, rest = (int64_t)p.D * (p.N + 2);
     const int64_t nb_bc = (bc + 255) / 256;
-    ADN_CHECK(nb_bc + (rest + 255) / 256 < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
     hipLaunchKernelGGL((scan_reduce_kernel<T, NS>), dim3((unsigned)(nb_bc + (rest + 255) / 256)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
                        a.dA, a.dD, a.ddelta_bias, p, (int)nb_bc);
     ADN_HIP_CHECK(hipGetLastError());
@@ -981,7 +980,7 @@ extern "C" int adn_op_selective_scan_forward(const adn_scan_args* a, void* hip_s
               "adn_op_selective_scan_forward: checkpoints smaller than adn_op_selective_scan_checkpoints() floats, or not on 16 bytes");
     ADN_CHECK(q.local == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= q.local + q.dsum), ADN_ERR_INVALID,
               "adn_op_selective_scan_forward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
-    ADN_CHECK((int64_t)a->batch * q.chunks * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_forward: batch too large");
+    ADN_CHECK(grid_ok((int64_t)a->batch * q.chunks * q.bpg * a->groups), ADN_ERR_INVALID, "adn_op_selective_scan_forward: batch too large");
     ScanParams p = params(*a, q);
     p.local = a->workspace;
     p.dsum = a->workspace + q.local;
@@ -999,7 +998,9 @@ extern "C" int adn_op_selective_scan_backward(const adn_scan_args* a, void* hip_
     const int64_t need = q.part_a + q.part_bc + q.local + q.dsum;
     ADN_CHECK(need == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= need), ADN_ERR_INVALID,
               "adn_op_selective_scan_backward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
-    ADN_CHECK((int64_t)q.nbg * q.chunks * q.bpg * a->groups < (int64_t)1 << 31, ADN_ERR_INVALID, "adn_op_selective_scan_backward: batch too large");
+    const int64_t sums = (int64_t)a->batch * a->steps * a->groups * a->states * 2 + (int64_t)a->channels * (a->states + 2);
+    ADN_CHECK(grid_ok((int64_t)q.nbg * q.chunks * q.bpg * a->groups) && grid_ok(sums / 256 + 2), ADN_ERR_INVALID,
+              "adn_op_selective_scan_backward: batch too large");
     ScanParams p = params(*a, q);
     p.local = a->workspace;
     p.dsum = p.local + q.local;
@@ -1013,6 +1014,7 @@ extern "C" int adn_op_selective_scan_step(const adn_scan_args* a, void* hip_stre
     if (a->batch == 0) return ADN_OK;
     ADN_CHECK(a->steps == 1 && !a->lens, ADN_ERR_INVALID, "adn_op_selective_scan_step: one frame, no lengths");
     ADN_CHECK(a->state_out, ADN_ERR_INVALID, "adn_op_selective_scan_step: null state");
+    ADN_CHECK(grid_ok((int64_t)a->batch * a->channels / 64 + 1), ADN_ERR_INVALID, "adn_op_selective_scan_step: batch * channels too large");
     const Plan q = plan_of(a->batch, 1, a->channels, a->states, a->groups, false);
     return dispatch<kStep>(*a, params(*a, q), q.ns, static_cast<hipStream_t>(hip_stream));
 }

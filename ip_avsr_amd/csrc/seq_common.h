@@ -87,6 +87,9 @@ struct SumSegs { float* out[kMaxSumSegs]; int64_t n[kMaxSumSegs]; int count; };
 // out[c] = sum over p < parts of ws[p * stride + c], p in a fixed order (layernorm.hip)
 int sum_parts(const float* ws, int64_t stride, int parts, const SumSegs& segs, hipStream_t s);
 
+// a launch of `blocks` workgroups of up to 256 threads along x stays below the 2^32 threads of a dimension
+static inline bool grid_ok(int64_t blocks) { return blocks < (int64_t)1 << 24; }
+
 // dense channels, element-aligned pointer, strides that do not overlap rows are the caller's promise; this checks what can be
 static inline bool seq_ok(const adn_seq& s, int elem) { return s.data && reinterpret_cast<uintptr_t>(s.data) % elem == 0; }
 static inline bool seq_aligned(const adn_seq& s, int elem, int bytes) {

@@ -61,6 +61,8 @@ def _first(name, x, dims):
         _fail("%s must be float32 or bfloat16, got %s" % (name, x.dtype))
     if x.dim() not in dims:
         _fail("%s must have %s dimensions, got %d" % (name, " or ".join(str(d) for d in dims), x.dim()))
+    if x.numel() >= 1 << 31 and max(x.shape) >= 1 << 31:          # (the library's sizes are 32-bit, and ctypes would cut them off)
+        _fail("a dimension of %s reaches 2^31" % name)
 
 
 def _call(fn, args, x):
@@ -218,7 +220,7 @@ def _scan_head(u, delta, A, Bm, Cm, D, z, delta_bias, lens, softplus, steps):
 
 
 def selective_scan_forward(u, delta, A, Bm, Cm, D=None, z=None, delta_bias=None, state=None, lens=None, softplus=True, save=False):
-    """The selective scan over ``u``, ``delta`` (batch, time, channels) with decays ``A`` (channels, states <= 32) and input / output
+    """The selective scan over ``u``, ``delta`` (batch, time, channels) with decays ``A`` (channels, states <= 32; finite) and input / output
     rows ``Bm``, ``Cm`` (batch, time, states) or (batch, time, groups, states)::
 
         dt = softplus(delta + delta_bias)          (softplus=False: the sum itself)

@@ -579,6 +579,11 @@ def test_sizes_that_the_library_refuses(S):
         S.layer_norm_backward(x, x, None, torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, device="cuda"))
     with pytest.raises(AdenetError, match="eps"):
         S.layer_norm_forward(x[..., :8].contiguous(), eps=-1.0)
+    long = torch.zeros(1, 1, 1, device="cuda").expand(1, (1 << 31) + 8, 1)
+    for fn in (S.layer_norm_forward, lambda v: S.causal_conv_forward(v, torch.ones(2, 1, device="cuda")),
+               lambda v: S.selective_scan_forward(v, v, -torch.ones(1, 1, device="cuda"), v, v)):
+        with pytest.raises(ValueError, match=r"2\^31"):
+            fn(long)
 
 
 def _random_lens(d, B, T):

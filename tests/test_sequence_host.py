@@ -77,7 +77,7 @@ def test_layer_norm_backward_refusals(lib):
 
 @pytest.mark.parametrize("over,word", [
     (dict(dtype=-1), "dtype"), (dict(taps=0), "taps"), (dict(taps=9), "taps"), (dict(activation=2), "activation"), (dict(weight=None), "weight"),
-    (dict(steps=-1), "steps"), (dict(channels=0), "channels"), (dict(x=None), "tensor"), (dict(state_out=None), "state_out"), (dict(state=64), "state_out")])
+    (dict(steps=-1), "steps"), (dict(channels=0), "channels"), (dict(x=None), "tensor"), (dict(state_out=None), "state_out"), (dict(state=64), "state_out"), (dict(batch=1 << 28, steps=1), "batch too large")])
 def test_causal_conv_refusals(lib, over, word):
     _refused(lib.adn_op_causal_conv_forward, _conv(**over), word, lib)
 
@@ -114,6 +114,8 @@ def test_selective_scan_backward_and_step_refusals(lib):
     _refused(back, _scan(**full, z=64, checkpoint_floats=n, workspace_floats=m), "gradient", lib)         # a gate without dz
     _refused(lib.adn_op_selective_scan_step, _scan(steps=2), "one frame", lib)
     _refused(lib.adn_op_selective_scan_step, _scan(steps=1, state_out=None), "state", lib)
+    _refused(lib.adn_op_selective_scan_step, _scan(steps=1, batch=1 << 21, channels=1 << 9), "too large", lib)
+    _refused(lib.adn_op_selective_scan_forward, _scan(batch=1 << 24, steps=1), "too large", lib)
     assert lib.adn_op_selective_scan_checkpoints(2, 3, 8, 33, 1) < 0 and lib.adn_op_selective_scan_workspace(2, 3, 8, 4, 3, 1) < 0
 
 
