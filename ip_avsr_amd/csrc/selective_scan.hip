@@ -723,25 +723,33 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
         (which ? dC : dB)[o] = (T)a;
         return;
     }
-    const int64_t i = (int64_t)(blockIdx.x - nb_bc) * 256 + threadIdx.x, da = (int64_t)p.D * p.N;
-    if (i >= da + 2 * (int64_t)p.D) return;
-    const int c = (int)(i < da ? i / p.N : (i - da) % p.D), n = (int)(i % p.N);
-    const int g = c / p.Dg, cg = c - g * p.Dg, tg = cg / WC, cw = cg % WC;
+    // 32 results x 8 lanes: lane k adds parts k, k + 8, ... and the eight sums are added in order
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t i = (int64_t)(blockIdx.x - nb_bc) * 32 + lane, da = (int64_t)p.D * p.N;
+    const bool on = i < da + 2 * (int64_t)p.D;
+    const int c = on ? (int)(i < da ? i / p.N : (i - da) % p.D) : 0, n = (int)(i % p.N);
+    const int g = c / p.Dg, cg = c - g * p.Dg, tg = cg / WC, cw = cg % WC, parts = p.nbg * p.chunks;
     const int64_t row = (int64_t)(g * p.bpg * 4 + tg) * (64 * P + 2 * WC), stride = (int64_t)p.ctiles * (64 * P + 2 * WC);
     int64_t at;
     if (i < da) {
-        const int lane = cw / NC * 4 + n / NS, m = cw % NC * NS + n % NS;
-        at = (m / 4 * 64 + lane) * 4 + m % 4;
+        const int lane_of = cw / NC * 4 + n / NS, m = cw % NC * NS + n % NS;
+        at = (m / 4 * 64 + lane_of) * 4 + m % 4;
     } else
         at = 64 * P + (i - da >= p.D ? WC : 0) + cw;
-    const float a = strided_sum(p.part_a + row + at, stride, p.nbg * p.chunks);
-    if (i < da) dA[i] = a;
-    else if (i - da < p.D) dD[c] = a;
-    else dbias[c] = a;
+    red[k][lane] = on ? strided_sum(p.part_a + row + at + k * stride, 8 * stride, (parts - k + 7) / 8) : 0.f;
+    __syncthreads();
+    if (k || !on) return;
+    float v = red[0][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v += red[w][lane];
+    if (i < da) dA[i] = v;
+    else if (i - da < p.D) dD[c] = v;
+    else dbias[c] = v;
 }
 
-// one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane; VEC: N = 4 NS and
-// everything aligned for NS values at a time.  Bound by the state's bytes, in and out
+// one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane; VEC: N in whole
+// vectors of min(NS, 4) states and everything aligned for them.  Bound by the state's bytes, in and out
 template <typename T, int NS, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u, int64_t ldu, const T* __restrict__ delta, int64_t ldd, const T* __restrict__ bm,
                                                         int64_t ldb, const T* __restrict__ cm, int64_t ldc, const T* __restrict__ z, int64_t ldz,
@@ -758,11 +766,20 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u,
     const T* br = bm + b * ldb + (int64_t)g * p.N;
     const T* cr = cm + b * ldc + (int64_t)g * p.N;
     float acc = 0.f, hv[NS], av[NS], bv[NS], cv[NS];
+    constexpr int W = NS < 4 ? NS : 4;
     if constexpr (VEC) {
-        load_vec<float, NS>(h + ng * NS, hv);
-        load_vec<float, NS>(p.A + (int64_t)c * p.N + ng * NS, av);
-        load_vec<T, NS>(br + ng * NS, bv);
-        load_vec<T, NS>(cr + ng * NS, cv);
+#pragma unroll
+        for (int j = 0; j < NS; j += W) {
+            const int n = ng * NS + j;
+            if (n < p.N) {
+                load_vec<float, W>(h + n, hv + j);
+                load_vec<float, W>(p.A + (int64_t)c * p.N + n, av + j);
+                load_vec<T, W>(br + n, bv + j);
+                load_vec<T, W>(cr + n, cv + j);
+            } else
+#pragma unroll
+                for (int i = 0; i < W; ++i) hv[j + i] = av[j + i] = bv[j + i] = cv[j + i] = 0.f;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -779,8 +796,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u,
         hv[j] = fmaf(__builtin_amdgcn_exp2f(dt * (av[j] * kLog2e)), hv[j], dtu * bv[j]);
         acc = fmaf(hv[j], cv[j], acc);
     }
-    if constexpr (VEC) store_vec<float, NS>(h + ng * NS, hv);
-    else
+    if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < NS; j += W)
+            if (ng * NS + j < p.N) store_vec<float, W>(h + ng * NS + j, hv + j);
+    } else
 #pragma unroll
         for (int j = 0; j < NS; ++j)
             if (ng * NS + j < p.N) h[ng * NS + j] = hv[j];
@@ -913,7 +933,7 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
 #undef ADN_SCAN_GO
     const int64_t bc = (int64_t)p.B * p.T * p.G * p.N * 2, rest = (int64_t)p.D * (p.N + 2);
     const int64_t nb_bc = (bc + 255) / 256;
-    hipLaunchKernelGGL((scan_reduce_kernel<T, NS>), dim3((unsigned)(nb_bc + (rest + 255) / 256)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
+    hipLaunchKernelGGL((scan_reduce_kernel<T, NS>), dim3((unsigned)(nb_bc + (rest + 31) / 32)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),
                        a.dA, a.dD, a.ddelta_bias, p, (int)nb_bc);
     ADN_HIP_CHECK(hipGetLastError());
     return ADN_OK;
@@ -922,8 +942,9 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
 template <typename T, int NS> int step(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
     const int64_t items = (int64_t)p.B * p.D;
     const int e = sizeof(T);
-    const auto rows = [&](const adn_seq& t) { return ptr_aligned(t.data, NS * e) && t.stride_b % NS == 0; };
-    const bool vec = p.N == 4 * NS && ptr_aligned(p.A, 16) && ptr_aligned(p.state_out, 16) && rows(a.b) && rows(a.c);
+    constexpr int W = NS < 4 ? NS : 4;
+    const auto rows = [&](const adn_seq& t) { return ptr_aligned(t.data, W * e) && t.stride_b % W == 0; };
+    const bool vec = p.N % W == 0 && ptr_aligned(p.A, 16) && ptr_aligned(p.state_out, 16) && rows(a.b) && rows(a.c);
 #define ADN_SCAN_GO(VEC)                                                                                                                           \
     hipLaunchKernelGGL((scan_step_kernel<T, NS, VEC>), dim3((unsigned)((items + 63) / 64)), dim3(256), 0, s, static_cast<const T*>(a.u.data), a.u.stride_b, \
                        static_cast<const T*>(a.delta.data), a.delta.stride_b, static_cast<const T*>(a.b.data), a.b.stride_b, static_cast<const T*>(a.c.data), \
@@ -998,7 +1019,7 @@ extern "C" int adn_op_selective_scan_backward(const adn_scan_args* a, void* hip_
     const int64_t need = q.part_a + q.part_bc + q.local + q.dsum;
     ADN_CHECK(need == 0 || (a->workspace && ptr_aligned(a->workspace, 16) && a->workspace_floats >= need), ADN_ERR_INVALID,
               "adn_op_selective_scan_backward: workspace smaller than adn_op_selective_scan_workspace() floats, or not on 16 bytes");
-    const int64_t sums = (int64_t)a->batch * a->steps * a->groups * a->states * 2 + (int64_t)a->channels * (a->states + 2);
+    const int64_t sums = (int64_t)a->batch * a->steps * a->groups * a->states * 2 + (int64_t)a->channels * (a->states + 2) * 8;
     ADN_CHECK(grid_ok((int64_t)q.nbg * q.chunks * q.bpg * a->groups) && grid_ok(sums / 256 + 2), ADN_ERR_INVALID,
               "adn_op_selective_scan_backward: batch too large");
     ScanParams p = params(*a, q);
