@@ -709,12 +709,13 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
     using L = Place<NS>;
     constexpr int P = L::P, WC = L::WC, NC = L::NC, SEG = L::SEG, STAGE = L::STAGE;
     if ((int)blockIdx.x < nb_bc) {
-        const int64_t gn = (int64_t)p.G * p.N, total = (int64_t)p.B * p.T * gn * 2;
-        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        if (i >= total) return;
-        const int which = i >= total / 2;
-        const int64_t o = i - (which ? total / 2 : 0), bt = o / gn;
-        const int n = (int)(o % p.N), g = (int)(o % gn) / p.N, b = (int)(bt / p.T), t = (int)(bt % p.T);
+        // fewer than 2^32 of them (the launch's limit), B's first
+        const unsigned gn = (unsigned)p.G * (unsigned)p.N, half = (unsigned)p.B * (unsigned)p.T * gn;
+        const unsigned i = blockIdx.x * 256 + threadIdx.x;
+        if (i >= 2 * half) return;
+        const int which = i >= half;
+        const unsigned o = i - (which ? half : 0), bt = o / gn, r = o - bt * gn;
+        const int g = (int)(r / (unsigned)p.N), n = (int)(r - (unsigned)g * (unsigned)p.N), b = (int)(bt / (unsigned)p.T), t = (int)(bt - (unsigned)b * (unsigned)p.T);
         float a = 0.f;
         if (t < valid_steps(p.lens, b, p.T)) {
             const float* src = p.part_bc + (((int64_t)b * p.nseg + t / SEG) * p.G + g) * STAGE + (t % SEG) * 8 * NS + which * 4 * NS + n;
