@@ -18,7 +18,13 @@ template <typename T> static inline View<const T> cview(const adn_seq& s) { retu
 
 template <typename T, int V> using vec_t = T __attribute__((ext_vector_type(V)));
 
-template <typename T, int V> __device__ __forceinline__ vec_t<T, V> load_raw(const T* __restrict__ p) { return *reinterpret_cast<const vec_t<T, V>*>(p); }
+// vectors at any element's address: rows of an odd width start off every wider alignment, and the hardware takes that
+template <typename T, int V> __device__ __forceinline__ vec_t<T, V> load_raw(const T* __restrict__ p) {
+    vec_t<T, V> v;
+    __builtin_memcpy(&v, p, sizeof(T) * V);
+    return v;
+}
+template <typename T, int V> __device__ __forceinline__ void store_raw(T* __restrict__ p, const vec_t<T, V>& v) { __builtin_memcpy(p, &v, sizeof(T) * V); }
 template <typename T, int V> __device__ __forceinline__ void widen(const vec_t<T, V>& v, float* out) {
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = (float)v[i];
@@ -40,7 +46,7 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T* __rest
         vec_t<T, V> v;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (T)in[i];
-        *reinterpret_cast<vec_t<T, V>*>(p) = v;
+        store_raw<T, V>(p, v);
     }
 }
 

@@ -156,6 +156,20 @@ def test_causal_conv(S, dtype, layout, carried, shape, taps, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,wide", [(9, 16), (65, 72), (1021, 1024), (1025, 1032)])
+def test_causal_conv_of_odd_widths_gives_the_bits_of_the_wider_one(S, dtype, D, wide):
+    torch = _torch()
+    d = Draw(("conv width", D), dtype)
+    (_, x), (_, dy), (_, w), (_, b), (_, st) = d.seq(3, 21, wide), d.seq(3, 21, wide), d.param(4, wide), d.param(wide), d.seq(3, 3, wide)
+    lens = _lens([21, 2, 13])
+    cut = [t[..., :D].contiguous() for t in (x, dy, w, b, st)]
+    whole = S.causal_conv_forward(x, w, b, state=st, lens=lens) + S.causal_conv_backward(dy, x, w, b, state=st, lens=lens)
+    part = S.causal_conv_forward(cut[0], cut[2], cut[3], state=cut[4], lens=lens) + S.causal_conv_backward(cut[1], cut[0], cut[2], cut[3], state=cut[4], lens=lens)
+    for got, want in zip(part, whole):
+        assert torch.equal(got, want[..., :D])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,D,taps", [(1, 1, 1), (3, 50, 4), (2, 2048, 4), (5, 33, 8), (70, 64, 2)])
 def test_causal_conv_step_continues_the_sequence(S, dtype, B, D, taps):
     d = Draw(("conv step", B, D, taps), dtype)
