@@ -169,6 +169,13 @@ template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p,
 template <int P> __device__ __forceinline__ int64_t local_at(const ScanParams& p, int b, int chunk, int ctile) {
     return (((int64_t)b * p.chunks + chunk) * p.ctiles + ctile) * 64 * P;
 }
+// x 2^e, finite wherever the product is: a scan that grows (A > 0, or steps below 0) may take a tiny x through more than 2^128, and
+// what it grows by on a zero is no infinity.  The whole part of e goes on behind the product; 400 is past any pair of float32 numbers
+__device__ __forceinline__ float times_exp2(float x, float e) {
+    e = fminf(fmaxf(e, -400.f), 400.f);
+    const float whole = rintf(e);
+    return __builtin_ldexpf(x * __builtin_amdgcn_exp2f(e - whole), (int)whole);
+}
 // x (a state, or a state's gradient) carried over a piece: x = what the piece alone leaves + exp(A sum dt) x
 template <int NS>
 __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>& l, int b, int chunk, const float (&A2)[Place<NS>::NC][NS],
@@ -181,7 +188,7 @@ __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>&
     for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(src + m * 256, v + m * 4);
     load_vec<float, NC>(ds, d);
 #pragma unroll
-    for (int m = 0; m < P; ++m) x[m / NS][m % NS] = fmaf(__builtin_amdgcn_exp2f(d[m / NS] * A2[m / NS][m % NS]), x[m / NS][m % NS], v[m]);
+    for (int m = 0; m < P; ++m) x[m / NS][m % NS] = v[m] + times_exp2(x[m / NS][m % NS], d[m / NS] * A2[m / NS][m % NS]);
 }
 
 // first launch over a split time axis: a piece alone.  Forward (BACK = false) the state it leaves, from zeros -- the first piece from the

@@ -23,7 +23,7 @@ class R(object):
         self.e = np.zeros_like(self.v) if e is None else np.broadcast_to(e, self.v.shape)
 
     def _round(self, v, e, n=1):
-        return R(v, e + n * U * np.abs(v) + _TINY)
+        return R(v, e + n * U * np.abs(v) + np.where((v != 0) | (e > 0), _TINY, 0.0))        # (exact zeros stay exact)
 
     def __add__(self, o):
         o = o if isinstance(o, R) else R(o)
@@ -56,8 +56,8 @@ class R(object):
         return R(self.v.sum((0, 1)), self.e.sum((0, 1)) + n * U * np.abs(self.v).sum((0, 1)))
 
     def exp(self):
-        v = np.exp(self.v)
-        return R(v, v * (self.e + 3 * U * np.abs(self.v) + 4 * U) + _TINY)
+        v = np.exp(self.v)               # far below float32's range both are zero
+        return R(v, v * (self.e + 3 * U * np.abs(self.v) + 4 * U) + np.where(self.v > -200, _TINY, 0.0))
 
     def sigmoid(self):
         v = np.where(self.v >= 0, 1 / (1 + np.exp(-np.abs(self.v))), np.exp(-np.abs(self.v)) / (1 + np.exp(-np.abs(self.v))))

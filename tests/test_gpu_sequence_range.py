@@ -1,0 +1,100 @@
+"""The sequence operators where values reach the ends of float32's range: scans that grow, decays of the type's lowest value, and
+infinities or NaN beside frames that are padding."""
+import numpy as np
+import pytest
+
+from oracle import sequence_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def S():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from ip_avsr_amd.custom import sequence
+    return sequence
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _near(name, got, want, dtype="float32"):
+    """Finite, and within twice the oracle's bound and half a step of the type (the oracle's header says why)."""
+    g = got.double().cpu().numpy()
+    assert g.shape == want.v.shape, (name, g.shape, want.v.shape)
+    assert np.isfinite(g).all(), "%s: %d values are not finite, the first at %s" % (name, (~np.isfinite(g)).sum(), np.argwhere(~np.isfinite(g))[0])
+    tol = 2 * want.e + O.HALF_STEP[dtype] * np.abs(want.v) * 1.01 + 1e-37
+    off = np.abs(g - want.v)
+    worst = (off / tol).max() if off.size else 0.0
+    assert worst <= 1.0, "%s: %.2f times the bound at %s" % (name, worst, np.unravel_index((off / tol).argmax(), off.shape))
+
+
+def _dev(x, dtype="float32"):
+    """(float64 values exact in `dtype`, device tensor)"""
+    torch = _torch()
+    t = torch.tensor(np.asarray(x, np.float32), device="cuda").to(getattr(torch, dtype))
+    return t.double().cpu().numpy(), t
+
+
+def _both(pairs):
+    return {k: p[0] for k, p in pairs.items()}, {k: p[1] for k, p in pairs.items()}
+
+
+def _check_scan(S, v, t, dy, dl, lens, dtype, softplus):
+    torch = _torch()
+    want = O.selective_scan(dy=dy[0], dlast=dl[0], lens=lens, softplus=softplus, **v)
+    for name in ("y", "state", "du", "ddelta", "dA", "dB", "dC", "dstate"):
+        assert np.abs(want[name].v).max() < 1e38, name                # (the case itself stays inside the type)
+    more = dict(lens=None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda"), softplus=softplus)
+    y, state, saved = S.selective_scan_forward(save=True, **t, **more)
+    _near("y", y, want["y"], dtype)
+    _near("state", state, want["state"])
+    g = S.selective_scan_backward(dy[1], saved=saved, dlast=dl[1], **t, **more)
+    for name in ("du", "ddelta", "dB", "dC"):
+        _near(name, g[name], want[name], dtype)
+    for name in ("dA", "dD", "ddelta_bias", "dstate"):
+        _near(name, g[name], want[name])
+    return want
+
+
+# states, channels, groups: 1, 2, 4 and 8 states per lane; 300 x 8: several workgroups along the channels
+GROWTH = [(3, 70, 1), (8, 40, 2), (16, 24, 1), (8, 300, 1), (32, 12, 1)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("N,D,G", GROWTH)
+def test_a_scan_that_grows_past_float32_within_a_piece_of_the_time_axis(S, dtype, softplus, N, D, G):
+    """Two utterances, long enough for a time axis in pieces (of 32 or 64 frames).  The first starts from states of 1e-18 and grows by
+    e^120 within 32 frames, the gradient of its last state, 1e-30, likewise on the way back: every h and dh is a float32 number, e^120 is
+    none.  The second grows by e^3.75 a frame throughout, from zeros: its input comes in the last 20 frames, its gradient leaves in
+    the first 10."""
+    rng = np.random.default_rng([41, N, D, softplus])
+    B, T, up = 2, 256, 3.75
+    lens = [T, T - 3]
+    assert S._lib.load().adn_op_selective_scan_workspace(B, T, D, N, G, 0) > 0      # pieces
+    logs = np.full((B, T), 1e-3)                       # log of the growth of a frame
+    logs[0, 64:96] = up
+    logs[1] = up
+    if softplus:       # dt = softplus(delta), A = 1 (to 0.1 %)
+        delta, sign = np.log(np.expm1(logs)), 1.0
+    else:              # dt < 0, A = -1
+        delta, sign = -logs, -1.0
+    u = rng.normal(size=(B, T, D))
+    u[0, :192] = 0
+    u[1, :T - 3 - 20] = 0
+    dy = rng.normal(size=(B, T, D))
+    dy[0, 48:] = 0                                      # (behind the growth: the gradient of the last state alone)
+    dy[1, 10:] = 0
+    state, dlast = 1e-18 * rng.normal(size=(B, D, N)), 1e-30 * rng.normal(size=(B, D, N))
+    state[1] = dlast[1] = 0
+    v, t = _both(dict(u=_dev(u, dtype), delta=_dev(np.broadcast_to(delta[..., None], (B, T, D)), dtype), A=_dev(sign * (1 + 1e-3 * rng.uniform(-1, 1, (D, N)))),
+                      Bm=_dev(rng.normal(size=(B, T, G, N)), dtype), Cm=_dev(rng.normal(size=(B, T, G, N)), dtype), D=_dev(rng.normal(size=D)), state=_dev(state)))
+    want = _check_scan(S, v, t, _dev(dy, dtype), _dev(dlast), lens, dtype, softplus)
+    # it grew, and the bound still says something
+    assert np.abs(want["state"].v).max() > 1e20 and np.abs(want["dstate"].v).max() > 1e15
+    assert np.median(want["state"].e / np.abs(want["state"].v)) < 1e-2
