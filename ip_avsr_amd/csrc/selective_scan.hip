@@ -79,6 +79,14 @@ __device__ __forceinline__ float softplusf(float x) {
     return fmaxf(x, 0.f) + 2.f * s * r;
 }
 
+// A as the exponent's factor for base 2.  The product passes float32's range from |A| = 2.36e38 on (the lowest value is what a state that
+// keeps nothing has), and an infinity times a step size of 0, or times a gradient of 0, would be NaN: the largest number has the same decays
+// (and the derivative by a step size of 0 is that of 2.36e38)
+__device__ __forceinline__ float decay2(float A) {
+    const float v = A * kLog2e;
+    return __builtin_isinf(v) ? __builtin_copysignf(3.40282347e38f, v) : v;
+}
+
 __device__ __forceinline__ float bcast(float v, int q) {
     switch (q) {
         case 0: return quad_bcast<0>(v);
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
         for (int j = 0; j < NS; ++j) {
             const int c = l.c0 + k, n = l.ng * NS + j;
             const bool on = c < l.cend && n < p.N;
-            A2[k][j] = on ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            A2[k][j] = on ? decay2(p.A[(int64_t)c * p.N + n]) : 0.f;
             h[k][j] = !BACK && on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
     const float bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
@@ -327,7 +335,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
         for (int j = 0; j < NS; ++j) {
             const int c = l.c0 + k, n = l.ng * NS + j;
             const bool on = c < l.cend && n < p.N;
-            A2[k][j] = on ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            A2[k][j] = on ? decay2(p.A[(int64_t)c * p.N + n]) : 0.f;
             h[k][j] = on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
     if (s0 < nv)
@@ -507,7 +515,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             const int c = l.c0 + k, n = l.ng * NS + j;
-            A2[k][j] = c < l.cend && n < p.N ? p.A[(int64_t)c * p.N + n] * kLog2e : 0.f;
+            A2[k][j] = c < l.cend && n < p.N ? decay2(p.A[(int64_t)c * p.N + n]) : 0.f;
             dA[k][j] = 0.f;
         }
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
@@ -801,7 +809,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u,
     }
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-        hv[j] = fmaf(__builtin_amdgcn_exp2f(dt * (av[j] * kLog2e)), hv[j], dtu * bv[j]);
+        hv[j] = fmaf(__builtin_amdgcn_exp2f(dt * decay2(av[j])), hv[j], dtu * bv[j]);
         acc = fmaf(hv[j], cv[j], acc);
     }
     if constexpr (VEC) {

@@ -98,3 +98,26 @@ def test_a_scan_that_grows_past_float32_within_a_piece_of_the_time_axis(S, dtype
     # it grew, and the bound still says something
     assert np.abs(want["state"].v).max() > 1e20 and np.abs(want["dstate"].v).max() > 1e15
     assert np.median(want["state"].e / np.abs(want["state"].v)) < 1e-2
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("T,N,D,lens", [(13, 5, 20, [13, 6]), (3, 3, 70, [1, 3]), (21, 16, 24, [9, 21]), (150, 8, 40, [150, 77]), (9, 32, 12, [5, 7])])
+def test_a_scan_with_decays_of_the_lowest_float32(S, T, N, D, lens, softplus):
+    """A = -3.4e38, a state that keeps nothing, also over frames that are padding and over steps of size 0; and single frames."""
+    torch = _torch()
+    rng = np.random.default_rng([42, T, N, D])
+    a = -np.exp(rng.normal(size=(D, N)))
+    a[rng.uniform(size=(D, N)) < 0.4] = np.finfo(np.float32).min
+    delta = rng.normal(size=(2, T, D)) if softplus else rng.uniform(0.1, 1, size=(2, T, D))
+    v, t = _both(dict(u=_dev(rng.normal(size=(2, T, D))), delta=_dev(delta), A=_dev(a), Bm=_dev(rng.normal(size=(2, T, 1, N))),
+                      Cm=_dev(rng.normal(size=(2, T, 1, N))), D=_dev(rng.normal(size=D)), state=_dev(rng.normal(size=(2, D, N)))))
+    want = _check_scan(S, v, t, _dev(rng.normal(size=(2, T, D))), _dev(rng.normal(size=(2, D, N))), lens, "float32", softplus)
+    low = v["A"] < -1e38
+    assert np.abs(want["dA"].v[low]).max() == 0 and np.abs(want["dA"].v[~low]).max() > 0
+    # a frame of step size 0 (a softplus far below float32's range, or the size itself) leaves every state as it is
+    h = t["state"].clone()
+    nothing = torch.full((2, D), -200.0 if softplus else 0.0, device="cuda")
+    S.selective_scan_step(t["u"][:, 0], nothing, t["A"], t["Bm"][:, 0], t["Cm"][:, 0], h, softplus=softplus)
+    assert torch.equal(h, t["state"])
+    one = {k: x[:, :1] for k, x in t.items() if k in ("u", "Bm", "Cm")}
+    assert torch.equal(S.selective_scan_forward(delta=nothing[:, None], A=t["A"], state=t["state"], softplus=softplus, **one)[1], t["state"])
