@@ -153,6 +153,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
             // frames: dx[t - (K - 1)] for t < t0 + K - 1 is then incomplete and belongs to the run before (or to the history).  Behind
             // the run's last frame, and behind the length, dpre adds to dx only, and behind the length it is zero
             const int stop = t1 + K - 1;
+            const int sum_end = min(t1, len);       // dpre is zero behind the length, but an infinity in the window would make that NaN
             for (int t = t0; t < stop; t += kConvChunk) {
                 float g[kConvChunk][V];
 #pragma unroll
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(View<const T> x, Vie
                         store_vec<T, V>(dx.row(b, s) + c, o);
                     } else if (s < 0 && p.dstate)
                         store_vec<T, V>(static_cast<T*>(p.dstate) + ((int64_t)b * (K - 1) + s + K - 1) * p.C + c, o);
-                    if (t + i < t1) {
+                    if (t + i < sum_end) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) {
                             const float d = pw[K - 1 + i][j];

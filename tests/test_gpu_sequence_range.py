@@ -121,3 +121,27 @@ def test_a_scan_with_decays_of_the_lowest_float32(S, T, N, D, lens, softplus):
     assert torch.equal(h, t["state"])
     one = {k: x[:, :1] for k, x in t.items() if k in ("u", "Bm", "Cm")}
     assert torch.equal(S.selective_scan_forward(delta=nothing[:, None], A=t["A"], state=t["state"], softplus=softplus, **one)[1], t["state"])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("D", [3, 8, 130])
+def test_frames_before_padding_stay_out_of_the_weight_gradient_of_padding(S, dtype, D):
+    """An infinity in the last frame of an utterance reaches the newest tap's gradient alone (the frames that the older taps would
+    take it to are padding), and what the history of an utterance of length 0 holds reaches none."""
+    torch = _torch()
+    rng = np.random.default_rng([43, D])
+    (_, x), (_, dy), (_, st) = (_dev(rng.normal(size=s), dtype) for s in ((4, 6, D), (4, 6, D), (4, 2, D)))
+    (_, w), (_, b) = _dev(rng.normal(size=(3, D))), _dev(rng.normal(size=D))
+    lens = torch.tensor([4, 6, 0, 5], dtype=torch.int32, device="cuda")
+    for act in ("linear", "silu"):
+        dx, dw, db, ds = S.causal_conv_backward(dy, x, w, b, state=st, lens=lens, activation=act)
+        odd = st.clone()
+        odd[2, 0], odd[2, 1] = float("nan"), float("inf")
+        for got, want in zip(S.causal_conv_backward(dy, x, w, b, state=odd, lens=lens, activation=act), (dx, dw, db, ds)):
+            assert torch.equal(got, want)
+    far = x.clone()
+    far[0, 3] = float("inf")
+    dx, dw, db, _ = S.causal_conv_backward(dy, x, w, b, state=st, lens=lens, activation="linear")
+    dx2, dw2, db2, _ = S.causal_conv_backward(dy, far, w, b, state=st, lens=lens, activation="linear")
+    assert torch.equal(dw[:2], dw2[:2]) and torch.equal(dx, dx2) and torch.equal(db, db2)
+    assert torch.equal(dw2[2], torch.sign(dy[0, 3].float()) * float("inf"))
