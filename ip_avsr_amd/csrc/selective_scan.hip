@@ -665,6 +665,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 if (GATED) odz[i] = gc[i] * (quad_gather(sy, l.b0, l.b1) + Dv * uc[i]) * sg * (1.f + zc[i] * (1.f - sg));
             }
             const auto rdu = wdu.base(t0), rdx = wdx.base(t0), rdz = wdz.base(t0);
+            if (!full)               // zeros for padding, also where an infinite state or gradient passes it
+#pragma unroll
+                for (int i = 0; i < Q; ++i)
+                    if (t0 + i * TQ + l.otp >= len) odu[i] = odz[i] = 0.f;
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
                 const bool on = t0 + i * TQ + l.otp < p.T;

@@ -145,3 +145,29 @@ def test_frames_before_padding_stay_out_of_the_weight_gradient_of_padding(S, dty
     dx2, dw2, db2, _ = S.causal_conv_backward(dy, far, w, b, state=st, lens=lens, activation="linear")
     assert torch.equal(dw[:2], dw2[:2]) and torch.equal(dx, dx2) and torch.equal(db, db2)
     assert torch.equal(dw2[2], torch.sign(dy[0, 3].float()) * float("inf"))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("T,N,D,lens", [(13, 5, 20, [13, 6]), (5, 3, 70, [1, 3]), (21, 16, 24, [9, 20]), (150, 8, 40, [150, 77]), (9, 32, 12, [5, 7])])
+def test_scan_gradients_of_padding_are_zeros_beside_infinities(S, dtype, value, T, N, D, lens):
+    """The gradient of the last state, or the first state, is infinite or NaN: frames that are padding still come back as zeros, and the
+    other utterance as if alone."""
+    torch = _torch()
+    rng = np.random.default_rng([44, T, N, D])
+    (_, u), (_, delta), (_, z), (_, dy) = (_dev(rng.normal(size=(2, T, D)), dtype) for _ in range(4))
+    (_, bm), (_, cm) = (_dev(rng.normal(size=(2, T, N)), dtype) for _ in range(2))
+    (_, A), (_, Dv), (_, h), (_, dl) = _dev(-np.exp(rng.normal(size=(D, N)))), _dev(rng.normal(size=D)), _dev(rng.normal(size=(2, D, N))), _dev(rng.normal(size=(2, D, N)))
+    more = dict(D=Dv, z=z, lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+
+    def passes(h, dl):
+        y, state, saved = S.selective_scan_forward(u, delta, A, bm, cm, state=h, save=True, **more)
+        g = S.selective_scan_backward(dy, u, delta, A, bm, cm, saved, state=h, dlast=dl, **more)
+        return dict(y=y, **{k: g[k] for k in ("du", "ddelta", "dz", "dB", "dC")})
+    plain = passes(h, dl)
+    for bad_h, bad_dl in ((False, True), (True, False)):
+        h2, dl2 = h.clone(), dl.clone()
+        (h2 if bad_h else dl2)[1] = value
+        for name, got in passes(h2, dl2).items():
+            assert not got[1, lens[1]:].any(), name
+            assert torch.equal(got[0], plain[name][0]), name
