@@ -1,10 +1,11 @@
 """The sequence operators' sums over frames, utterances and workgroups: exactly, on integers (oracle/sequence_integers.py says why float32
-computes them exactly)."""
+computes them exactly), and time axes in pieces over several workgroups of channels against the float64 oracle."""
 import numpy as np
 import pytest
 
 from oracle import sequence_integers as I
-from tests.test_gpu_sequence import _lens
+from oracle import sequence_oracle as O
+from tests.test_gpu_sequence import Draw, _lens, _near, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,26 @@ def test_selective_scan_exactly(S, dtype, shape, N, G):
     for name, got in dict(g, y=y, state=state).items():
         if name != "dz":
             _equal(name, got, want[name])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gated,carried,softplus", [(True, True, True), (False, False, True), (True, False, False)])
+@pytest.mark.parametrize("shape,N,G,lens", [((2, 150, 150), 16, 1, [150, 70]), ((1, 140, 300), 16, 2, [133]), ((1, 150, 130), 24, 1, [149]), ((2, 130, 300), 7, 1, [129, 40]),
+                                            ((1, 131, 520), 4, 2, None)], ids=str)
+def test_pieces_of_the_time_axis_over_several_workgroups(S, dtype, gated, carried, softplus, shape, N, G, lens):
+    B, T, D = shape
+    lib = S._lib.load()
+    assert lib.adn_op_selective_scan_workspace(B, T, D, N, G, 0) > 0
+    d = Draw(("pieces", shape, N, G, gated), dtype, "columns")
+    v, t = _scan_inputs(d, shape, N, G, lens, gated, softplus, carried)
+    dyv, dy = d.seq(*shape, lens=lens)
+    dlv, dl = d.param(B, D, N) if carried else (None, None)
+    want = O.selective_scan(dy=dyv, dlast=dlv, **v)
+    y, state, saved = S.selective_scan_forward(save=True, **t)
+    g = S.selective_scan_backward(dy, saved=saved, dlast=dl, **t)
+    _near("y", y, want["y"], dtype)
+    _near("state", state, want["state"])
+    for name in ("du", "ddelta", "dB", "dC") + (("dz",) if gated else ()):
+        _near(name, g[name], want[name], dtype)
+    for name in ("dA", "dD", "ddelta_bias") + (("dstate",) if carried else ()):
+        _near(name, g[name], want[name])
