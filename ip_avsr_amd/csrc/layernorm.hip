@@ -66,7 +66,8 @@ struct RowCursor {
 };
 template <int TPR> __device__ __forceinline__ int row_in_block() { return TPR == 64 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) : 0; }
 
-// a thread's part of the row under the cursor; zeros behind D, and for a row that is not there or padding
+// a thread's part of the row under the cursor, zeros behind D; `out` stays as it was for a row that is not there or padding (the callers
+// look at the cursor's `valid`)
 template <typename T, int V, int NV, int TPR>
 __device__ __forceinline__ void load_row(const View<const T>& x, const NormParams& p, const RowCursor& q, int l, vec_t<T, V> (&out)[NV]) {
     if (q.valid) {
@@ -332,8 +333,10 @@ template <typename T, int V, bool BWD> int launch(const adn_norm_args& a, const 
         else if (BWD || p.D <= 64 * 16) ADN_LN_GO(64, NV);
         else if constexpr (!BWD) ADN_LN_GO(64, (32 / V));
     } else if (tpr == 256) {
-        if (p.D <= 256 * 8) ADN_LN_GO(256, (8 / V));
-        else ADN_LN_GO(256, NV);
+        if (BWD && p.D <= 256 * 8) {      // (forward such a row is a wave's)
+            if constexpr (BWD) ADN_LN_GO(256, (8 / V));
+        } else
+            ADN_LN_GO(256, NV);
     } else if (tpr == 512)
         ADN_LN_GO(512, NV);
     else

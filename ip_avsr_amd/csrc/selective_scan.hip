@@ -49,7 +49,7 @@ struct ScanParams {
     float* part_bc;                   // backward: [bpg][B][nseg][G][SEG][2][4 NS]
     float* part_a;                    // backward: [nbg][chunks][ctiles][64 P + 2 * 16 NC]
     int B, T, D, N, G, Dg;            // Dg = D / G channels per group
-    int nseg, tpg, bpg, ctiles;       // segments; waves and workgroups per group; waves of all workgroups along the channels
+    int nseg, bpg, ctiles;            // segments; workgroups per group; waves of all workgroups along the channels
     int nbg, per_bg;                  // backward: groups of utterances, utterances per group
     int chunks, spc;                  // pieces that the time axis is split into, segments of a piece
     float* local;                     // chunks > 1: what a piece alone leaves, [B][chunks][ctiles][P / 4][64][4] ...
@@ -911,7 +911,7 @@ ScanParams params(const adn_scan_args& a, const Plan& q) {
     p.lens = a.lens; p.A = a.A; p.Dp = a.D; p.dbias = a.delta_bias; p.state_in = a.state; p.state_out = a.state_out; p.ckpt = a.checkpoints;
     p.dlast = a.dlast; p.dstate = a.dstate;
     p.B = a.batch; p.T = a.steps; p.D = a.channels; p.N = a.states; p.G = a.groups; p.Dg = a.channels / a.groups;
-    p.nseg = q.nseg; p.tpg = q.tpg; p.bpg = q.bpg; p.ctiles = q.ctiles; p.nbg = q.nbg; p.per_bg = q.per_bg;
+    p.nseg = q.nseg; p.bpg = q.bpg; p.ctiles = q.ctiles; p.nbg = q.nbg; p.per_bg = q.per_bg;
     p.chunks = q.chunks; p.spc = q.spc;
     p.softplus = a.softplus;
     return p;
