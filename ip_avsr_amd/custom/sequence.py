@@ -61,7 +61,7 @@ def _first(name, x, dims):
         _fail("%s must be float32 or bfloat16, got %s" % (name, x.dtype))
     if x.dim() not in dims:
         _fail("%s must have %s dimensions, got %d" % (name, " or ".join(str(d) for d in dims), x.dim()))
-    if x.numel() >= 1 << 31 and max(x.shape) >= 1 << 31:          # (the library's sizes are 32-bit, and ctypes would cut them off)
+    if not 0 < x.numel() < 1 << 31 and max(x.shape) >= 1 << 31:          # (the library's sizes are 32-bit, and ctypes would cut them off)
         _fail("a dimension of %s reaches 2^31" % name)
 
 
@@ -108,6 +108,10 @@ def layer_norm_backward(dy, x, gamma, mean, inv_std, lens=None):
     _first("x", x, (2, 3))
     if x.dim() == 2:
         _first("dy", dy, (2,))
+        for name, t in (("mean", mean), ("inv_std", inv_std)):
+            if t is None:
+                _fail("the backward pass needs %s" % name)
+            _param(name, t, x.shape[:1], x)
         dx, dgamma, dbeta = layer_norm_backward(dy[None], x[None], gamma, mean[None], inv_std[None], lens)
         return dx[0], dgamma, dbeta
     B, T, D = x.shape

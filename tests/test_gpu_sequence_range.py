@@ -171,3 +171,20 @@ def test_scan_gradients_of_padding_are_zeros_beside_infinities(S, dtype, value, 
         for name, got in passes(h2, dl2).items():
             assert not got[1, lens[1]:].any(), name
             assert torch.equal(got[0], plain[name][0]), name
+
+
+def test_refusals_of_bad_statistics_and_of_empty_tensors_with_a_dimension_of_2_31(S):
+    torch = _torch()
+    x = torch.randn(5, 8, device="cuda")
+    _, m, i = S.layer_norm_forward(x)
+    for mean, inv in ((None, i), (m, None), (1.0, i), (m[:4], i), (m, i.double()), (m, i.cpu())):
+        with pytest.raises(ValueError, match="mean|inv_std"):
+            S.layer_norm_backward(x, x, None, mean, inv)
+    none = x[:0]
+    assert not S.layer_norm_backward(none, none, None, m[:0], i[:0])[1].any()
+    # the library's sizes are 32-bit: (2^32 + 1, 0, 1) is not (1, 0, 1)
+    far = torch.empty((1 << 32) + 1, 0, 1, device="cuda")
+    one = torch.ones(1, 1, device="cuda")
+    for fn in (S.layer_norm_forward, lambda v: S.causal_conv_forward(v, one), lambda v: S.selective_scan_forward(v, v, -one, v, v)):
+        with pytest.raises(ValueError, match=r"2\^31"):
+            fn(far)
