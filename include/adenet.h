@@ -392,8 +392,10 @@ int adn_op_copy_bench(const float* src, float* dst, int64_t n, int repeats, void
  *    results are rounded once.  Outputs must not overlap inputs.
  *  - lens (int32 [B], or null: all frames): frames at and behind an utterance's length are padding -- never read, zero in every
  *    result, absent from every sum, and a state passes them unchanged.  Values outside [0, T] are clamped.
- *  - All sums run in a fixed order: the same bits on every run.  No frame, utterance or element count may reach 2^31 except where the
- *    tensor's byte size says otherwise (offsets are 64-bit).
+ *  - All sums run in a fixed order: the same bits on every run.
+ *  - Sizes: batch * steps below 2^31 - 65536; the scan's batch * channels below 2^31 (single frames: 2^30), its frame strides below
+ *    2^26 elements; channels up to 2^20 (layer norm 16384).  Calls of 2^24 workgroups or more are refused.  Offsets of frames and
+ *    utterances are 64-bit: a tensor may be larger than 4 GiB.
  * The *_workspace / *_checkpoints functions return a count of floats (< 0: sizes out of range); such buffers start on 16 bytes. */
 typedef enum { ADN_DTYPE_F32 = 0, ADN_DTYPE_BF16 = 1 } adn_dtype;
 typedef struct {

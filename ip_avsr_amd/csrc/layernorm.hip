@@ -7,8 +7,9 @@
 // then the centred second moment, so nothing cancels -- spread over 64, 256, 512 or 1024 threads (the fewest that keep it to 16 values
 // per thread, forward on one wave 32: more registers per thread cost the waves that hide the loads).  The workgroups are persistent:
 // gamma and beta stay in registers over all their rows, the next row's loads are in flight during a row's sums, and the backward pass adds dgamma / dbeta there too, leaves one partial row per workgroup, and a
-// second launch adds those in a fixed order -- the same bits on every run.  32768 x 4096 bfloat16: forward 94 us (5.7 TB/s), backward
-// 168 us (4.8 TB/s) and 6 us for the partial rows; 13520 of 20800 x 1000 float32: 29, 35 and 5 us.
+// second launch adds those in a fixed order -- the same bits on every run.  32768 x 4096 bfloat16: forward 96 us (5.6 TB/s), backward
+// 171 us (4.7 TB/s) and 6 us for the partial rows; 13520 of 20800 x 1000 float32: 29, 35 and 5 us.  Narrow rows leave most of a wave
+// idle: 10^6 rows of 50 float32 take 261 and 395 us (the memory 80 and 120), its two 64-lane sums a row being the limit.
 // Frames at and behind lens[b] are padding: not read, zero in every result, absent from the sums.
 #include "seq_common.h"
 
@@ -153,7 +154,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ln_backward_kernel(View
     __shared__ float red[2][2 * NW];                         // alternating rows: one barrier per row is then enough
     __shared__ float comb[TPR == 64 ? 2 * 64 * NV * V : 1];
     const int l = threadIdx.x % TPR;
-    // 1024 threads have 128 registers each: gamma is then read again for every row and the next row's loads wait
+    // 1024 threads have 128 registers each: gamma is then read again for every row and the next row's loads wait.  Even so some spill,
+    // 4 (bfloat16) and 9 with vectors, 88 and 60 without: 4096 x 16384 bfloat16 120 us (3.4 TB/s), x 16381 570 us (0.7)
     constexpr bool AHEAD = TPR < 1024;
     float gm[NV][V], dg[NV][V], db[NV][V];
     if (AHEAD) load_param<V, NV, TPR>(p.gamma, 1.f, p.D, l, gm);
@@ -288,7 +290,8 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 
 constexpr int kMaxNormChannels = 16 * 1024;
 
-constexpr int kNormBlocks = 1024;      // forward: four persistent workgroups per CU
+// forward: four persistent workgroups per CU; at 1025 .. 2048 channels (133 to 168 registers) three are resident and the fourth follows
+constexpr int kNormBlocks = 1024;
 // backward: workgroups, each of which leaves a partial row -- as many as are resident at once: one more round of fewer costs more than
 // idle CUs (32768 x 4096 bf16: 768 workgroups 168 us, 1024 184 us; 20800 x 2000: 1024 58 us, 768 65 us)
 int norm_parts(int64_t rows, int D, int tpr) {
@@ -349,6 +352,8 @@ template <typename T, int V, bool BWD> int launch(const adn_norm_args& a, const 
 template <bool BWD> int run(const adn_norm_args& a, const NormParams& p, hipStream_t s) {
     const bool bf = a.dtype == ADN_DTYPE_BF16;
     const int e = bf ? 2 : 4;
+    // vectors where rows and pointers keep to 16 bytes, else one element at a time: 20800 x 2000 at a column offset of 3 takes forward
+    // 80 us against 38 in bfloat16 and 80 against 75 in float32, backward 70 against 65 and 117 against 117
     const bool al = a.channels * e % 16 == 0 && ptr_aligned(a.gamma, 16) && (BWD || ptr_aligned(a.beta, 16)) && seq_aligned(a.x, e, 16) && (BWD ? seq_aligned(a.dy, e, 16) && seq_aligned(a.dx, e, 16) : seq_aligned(a.y, e, 16));
     if (bf) return al ? launch<__bf16, 8, BWD>(a, p, s) : launch<__bf16, 1, BWD>(a, p, s);
     return al ? launch<float, 4, BWD>(a, p, s) : launch<float, 1, BWD>(a, p, s);

@@ -21,9 +21,8 @@
 // registers, then runs the adjoint.  dB and dC are summed over the lanes of a wave by exchanging halves (permlane swaps, row
 // rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
 // over all frames of a workgroup's utterances.  All sums run in a fixed order.
-// 8 x 2048 x 2048 x 16 bfloat16, gated: forward 280 us with what training keeps, 0.52 us per 10^6 (t, d, n) where the 8 slots take 0.20
-// (1024 waves, one per SIMD: the issue of that one is the limit; with four per SIMD 0.33), backward 468 us (27 vector instructions a
-// (t, d, n), the pipe 83 % busy) behind 121 us for the pieces alone.
+// 8 x 2048 x 2048 x 16 bfloat16, gated: forward 285 us with what training keeps, 0.53 us per 10^6 (t, d, n) where the 8 slots take 0.20
+// (1024 waves, one per SIMD, the pipe 47 % busy: nothing covers a wave's own waits; with four per SIMD 0.33), backward 497 us (26 vector instructions a (t, d, n), the pipe 87 % busy) behind 131 us for the pieces alone.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
 #include <type_traits>
@@ -769,7 +768,8 @@ __global__ __launch_bounds__(256) void scan_reduce_kernel(T* __restrict__ dB, T*
 }
 
 // one frame of every utterance, the state moved on in place: a quad per channel, NS neighbouring states per lane; VEC: N in whole
-// vectors of min(NS, 4) states and everything aligned for them.  Bound by the state's bytes, in and out
+// vectors of min(NS, 4) states and everything aligned for them (321 x 2102 x 24: 27 us, state by state 75).  Bound by the state's
+// bytes, in and out
 template <typename T, int NS, bool VEC>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ u, int64_t ldu, const T* __restrict__ delta, int64_t ldd, const T* __restrict__ bm,
                                                         int64_t ldb, const T* __restrict__ cm, int64_t ldc, const T* __restrict__ z, int64_t ldz,
@@ -853,10 +853,13 @@ Plan plan_of(int64_t B, int64_t T, int D, int N, int G, bool bwd) {
     q.bpg = cdiv(q.tpg, 4);
     q.ctiles = q.bpg * G * 4;
     q.ckpt = B * q.nseg * q.ctiles * 64 * P;
-    // backward: enough groups of utterances for two workgroups per CU
+    // backward: groups of utterances for about 1024 workgroups, two rounds of the 512 that are resident (two waves per SIMD); rounding
+    // the group's size down can leave a few for a third round
     const int64_t want = std::max<int64_t>(1, cdiv(1024, q.bpg * G));
     q.per_bg = (int)std::max<int64_t>(1, B / want);
     q.nbg = cdiv(B, q.per_bg);
+    // (workgroups are whole, four waves: 64 channels of 16 states, 256 of up to 4.  A group of fewer channels runs waves that own none,
+    // and their states are kept too: 520 x 2000 x 16 channels of 4 states take 1.07 GB of checkpoints)
     // a time axis in pieces, where the utterances and channels alone are too few waves: the first launch costs 7 / 8 of the work once
     // more forward and a third of it backward.  512 frames x 2048 channels x 16 states, 768 waves: forward 60 against 70 us, 1024
     // waves: forward 76 against 72, backward 172 against 180 us

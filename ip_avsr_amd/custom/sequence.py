@@ -8,7 +8,7 @@ and, where it carries a state, a ``*_step`` for one frame of every utterance, wh
 
 Tensors are CUDA torch tensors, nothing is copied or converted: activations (batch, time, channels) in float32 or bfloat16, all of one
 call in the same type, with dense channels and any frame and utterance stride (column ranges of a wider projection, time-major
-arrays); parameters, statistics and the scan's states in float32, dense.  Results are new dense tensors.  ``lens`` (int32, one length
+arrays; the scan takes frame strides below 2^26 elements); parameters, statistics and the scan's states in float32, dense.  Results are new dense tensors.  ``lens`` (int32, one length
 per utterance) marks frames at and behind it as padding: never read, zero in every result, absent from every sum, and a state passes
 them unchanged; lengths outside [0, T] are clamped.  Work is enqueued on the current stream of the tensors' device; sums run in a
 fixed order, so two runs give the same bits.  A bad argument raises ``ValueError``, sizes that the library refuses ``AdenetError``;
