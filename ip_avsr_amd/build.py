@@ -13,9 +13,9 @@ LIB = os.path.join(CSRC, "libadenet_hip.so")
 
 
 def build(force=False, verbose=True):
+    cmd = ["make", "-C", CSRC, "-j", str(min(8, os.cpu_count() or 1))]
     if force:
-        subprocess.check_call(["make", "-C", CSRC, "clean"], stdout=subprocess.DEVNULL)
-    cmd = ["make", "-C", CSRC, "-j", str(min(4, os.cpu_count() or 1))]
+        cmd.append("-B")          # every source again; the library stays in place until the new one is linked
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or res.returncode:
         sys.stdout.write(res.stdout)
