@@ -453,9 +453,8 @@ int adn_op_causal_conv_step(const adn_conv_args* args, void* hip_stream);
 /* dt = softplus(delta + delta_bias) (softplus = 0: no softplus), h = exp(dt A) h + dt u B_t, y = sum_n h C_t + D u, y *= z sigmoid(z).
  * A float32 [channels][states] (finite), states <= 32; b and c: (B, T, groups * states), channel d reads group d / (channels / groups);
  * D, delta_bias float32 [channels] or null (0); z.data null: no gate; state float32 [B][channels][states] or null (zeros).
- * A scan may grow (A > 0, or steps below 0), as long as exp(dt A) of a frame and the states are float32 numbers.  A long time axis is
- * worked on in pieces, each from zeros first: where the input cancels a growth of a carried state past 2^127, of which float32 keeps no
- * digit, a result may be infinite or NaN that is finite frame by frame.
+ * A scan may grow (A > 0, or steps below 0), as long as exp(dt A) of a frame and the states are float32 numbers: a long time axis, which
+ * is worked on in pieces, is finite where it is frame by frame.
  * Training: the forward pass fills `checkpoints`, the backward pass reads them (same sizes, same lens) instead of `state`. */
 typedef struct {
     int32_t dtype, batch, steps, channels, states, groups, softplus, reserved;

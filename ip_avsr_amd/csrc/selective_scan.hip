@@ -176,15 +176,8 @@ template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p,
 template <int P> __device__ __forceinline__ int64_t local_at(const ScanParams& p, int b, int chunk, int ctile) {
     return (((int64_t)b * p.chunks + chunk) * p.ctiles + ctile) * 64 * P;
 }
-// x 2^e, finite wherever the product is: a scan that grows (A > 0, or steps below 0) may take a tiny x through more than 2^128, and
-// what it grows by on a zero is no infinity.  The whole part of e goes on behind the product; 400 is past any pair of float32 numbers
-__device__ __forceinline__ float times_exp2(float x, float e) {
-    e = fminf(fmaxf(e, -400.f), 400.f);
-    const float whole = rintf(e);
-    return __builtin_ldexpf(x * __builtin_amdgcn_exp2f(e - whole), (int)whole);
-}
 // x (a state, or a state's gradient) carried over a piece: x = what the piece alone leaves + exp(A sum dt) x
-template <int NS>
+template <int NS, bool CAREFUL>
 __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>& l, int b, int chunk, const float (&A2)[Place<NS>::NC][NS],
                                            float (&x)[Place<NS>::NC][NS]) {
     constexpr int P = Place<NS>::P, NC = Place<NS>::NC, WC = Place<NS>::WC;
@@ -195,7 +188,65 @@ __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>&
     for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(src + m * 256, v + m * 4);
     load_vec<float, NC>(ds, d);
 #pragma unroll
-    for (int m = 0; m < P; ++m) x[m / NS][m % NS] = v[m] + times_exp2(x[m / NS][m % NS], d[m / NS] * A2[m / NS][m % NS]);
+    for (int m = 0; m < P; ++m) {
+        const float e = d[m / NS] * A2[m / NS][m % NS];
+        if (CAREFUL) {
+            // a scan that grows (A > 0, or steps below 0) may take a tiny state through more than 2^128, and what it grows by on a zero is
+            // no infinity: a third of the exponent at a time, 127 of them at most (more is past any pair of numbers)
+            const float f = __builtin_amdgcn_exp2f(fminf(e * (1.f / 3.f), 127.f));
+            x[m / NS][m % NS] = fmaf(x[m / NS][m % NS] * f * f, f, v[m]);
+        } else
+            x[m / NS][m % NS] = fmaf(__builtin_amdgcn_exp2f(e), x[m / NS][m % NS], v[m]);
+    }
+}
+template <int NC, int NS> __device__ __forceinline__ bool all_finite(const float (&x)[NC][NS]) {
+    bool on = true;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) on = on && __builtin_isfinite(x[k][j]);
+    return on;
+}
+
+// The states (gradients) of a lane over the frames from .. to themselves, for where they do not come out finite over the pieces: a piece
+// alone can overflow that frame by frame would not, where its input cancels what an earlier state grows to.  States that are all NaN
+// end it: nothing changes them.  Backward (in: dy, m: C, z: the gate or null) from the end.
+template <typename T, int NS, bool BACK>
+__device__ __forceinline__ void over_frames(const View<const T>& in, const View<const T>& delta, const View<const T>& m, const View<const T>& z, const ScanParams& p,
+                                            const Place<NS>& l, int b, int from, int to, const float (&A2)[Place<NS>::NC][NS], float (&x)[Place<NS>::NC][NS]) {
+#pragma unroll 1
+    for (int i = from; i < to; ++i) {
+        const int t = BACK ? to - 1 - (i - from) : i;
+        bool live = false;
+#pragma unroll
+        for (int k = 0; k < Place<NS>::NC; ++k) {
+            const int c = l.c0 + k;
+            if (c >= l.cend) break;
+            const float d = (float)delta.row(b, t)[c] + (p.dbias ? p.dbias[c] : 0.f), dt = p.softplus ? softplusf(d) : d;
+            float v = (float)in.row(b, t)[c];
+            if (!BACK) v *= dt;
+            else if (z.p) { const float zv = (float)z.row(b, t)[c]; v *= zv * sigmoidf(zv); }
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const int n = l.ng * NS + j;
+                if (n >= p.N) break;
+                const float a = __builtin_amdgcn_exp2f(dt * A2[k][j]), mv = (float)m.row(b, t)[l.g * p.N + n];
+                x[k][j] = BACK ? a * fmaf(mv, v, x[k][j]) : fmaf(a, x[k][j], v * mv);
+                live = live || x[k][j] == x[k][j];
+            }
+        }
+        if (!live) break;
+    }
+}
+// x carried over the pieces that walk(carry) goes through: plainly, and where that is not finite (a scan that grows) from reset() again,
+// with care, and at last over the frames
+template <int NS, typename Walk, typename Reset, typename Frames>
+__device__ __forceinline__ void carry_all(float (&x)[Place<NS>::NC][NS], const Walk& walk, const Reset& reset, const Frames& frames) {
+    walk(std::false_type{});
+    if (all_finite(x)) return;
+    reset();
+    walk(std::true_type{});
+    if (!all_finite(x)) frames();
 }
 
 // first launch over a split time axis: a piece alone.  Forward (BACK = false) the state it leaves, from zeros -- the first piece from the
@@ -316,17 +367,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     if (l.otp == 0) p.dsum[(((int64_t)b * p.chunks + chunk) * p.ctiles + l.ctile) * WC + l.cl * NC + l.ng] = total;
 }
 
-template <typename T, int NS, bool GATED, bool SAVE>
+// PIECES: the time axis is split (an unsplit one has no carries, and no registers for them)
+template <typename T, int NS, bool GATED, bool SAVE, bool PIECES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
                                                            View<T> y, ScanParams p) {
     using L = Place<NS>;
     constexpr int NC = L::NC, TQ = L::TQ, P = L::P, Q = L::Q, SEG = L::SEG, STAGE = L::STAGE;
     __shared__ __align__(16) float bc[2][STAGE];
     const int cb = p.bpg * p.G;
-    const int item = (int)(blockIdx.x / cb), b = item / p.chunks, chunk = item - b * p.chunks;
+    const int item = (int)(blockIdx.x / cb), b = PIECES ? item / p.chunks : item, chunk = PIECES ? item - b * p.chunks : 0;
     const L l(p, (int)(blockIdx.x - (unsigned)item * cb));
     const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
-    const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc);
+    const int s0 = PIECES ? chunk * p.spc : 0, s1 = PIECES ? min(nv, s0 + p.spc) : nv;
     float A2[NC][NS], h[NC][NS];
 #pragma unroll
     for (int k = 0; k < NC; ++k)
@@ -335,10 +387,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             const int c = l.c0 + k, n = l.ng * NS + j;
             const bool on = c < l.cend && n < p.N;
             A2[k][j] = on ? decay2(p.A[(int64_t)c * p.N + n]) : 0.f;
-            h[k][j] = on && chunk == 0 && p.state_in ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
         }
-    if (s0 < nv)
-        for (int c = 0; c < chunk; ++c) carry_over<NS>(p, l, b, c, A2, h);
+    const auto first_states = [&](bool given) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                const int c = l.c0 + k, n = l.ng * NS + j;
+                h[k][j] = given && c < l.cend && n < p.N ? p.state_in[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+            }
+    };
+    first_states(chunk == 0 && p.state_in);
+    if (PIECES && s0 < nv && chunk > 0)
+        carry_all<NS>(h, [&](auto careful) { for (int c = 0; c < chunk; ++c) carry_over<NS, decltype(careful)::value>(p, l, b, c, A2, h); },
+                      [&] { first_states(false); },             // (the first piece alone begins with the states that are given)
+                      [&] { first_states(p.state_in); over_frames<T, NS, false>(u, delta, bm, View<const T>{}, p, l, b, 0, s0 * SEG, A2, h); });
     const float Dv = l.ocv && p.Dp ? p.Dp[l.oc] : 0.f, bias = l.ocv && p.dbias ? p.dbias[l.oc] : 0.f;
     int ft = s0 * SEG;
     Walk<const T> wu(u, b, ft, l.otp, l.oc, l.ocv), wx(delta, b, ft, l.otp, l.oc, l.ocv), wz(z, b, GATED ? ft : 0, l.otp, l.oc, l.ocv);
@@ -442,10 +505,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
             if (seg + 1 < s1) segment(seg + 1, odd);
         }
     }
-    const int end = min(p.T, (s0 + p.spc) * SEG);
+    const int end = PIECES ? min(p.T, (s0 + p.spc) * SEG) : p.T;
     for (int t = max(nv, s0) * SEG + l.otp; t < end; t += TQ)
         if (l.ocv) y.row(b, t)[l.oc] = (T)0.f;
-    if (chunk == max(nv - 1, 0) / p.spc)
+    if (!PIECES || chunk == max(nv - 1, 0) / p.spc)
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -496,7 +559,7 @@ template <int NS> __device__ __forceinline__ float reduce_quads(const float (&v)
     }
 }
 
-template <typename T, int NS, bool GATED>
+template <typename T, int NS, bool GATED, bool PIECES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void scan_backward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
                                                                View<const T> dy, View<T> du, View<T> ddelta, View<T> dz, ScanParams p) {
     using L = Place<NS>;
@@ -505,7 +568,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ __align__(16) float bc[2][STAGE];
     __shared__ float red[2][4][SEG][16 * NS];           // per frame 8 NS sums and 8 NS places nobody reads
     const int cb = p.bpg * p.G;
-    const int item = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)item * cb), bg = item / p.chunks, chunk = item - bg * p.chunks;
+    const int item = (int)(blockIdx.x / cb), cblk = (int)(blockIdx.x - (unsigned)item * cb), bg = PIECES ? item / p.chunks : item, chunk = PIECES ? item - bg * p.chunks : 0;
     const L l(p, cblk);
     const int red_at = reduced_at<NS>(l.lane);
     float A2[NC][NS], dA[NC][NS];
@@ -525,20 +588,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int i = threadIdx.x, s = i / (8 * NS), at = i % (8 * NS);
         if (i < STAGE) flush_at[i] = ((rd[0][s][at] + rd[1][s][at]) + rd[2][s][at]) + rd[3][s][at];
     };
-    const int b_end = min(p.B, (bg + 1) * p.per_bg);
-    for (int b = bg * p.per_bg; b < b_end; ++b) {
+    const int b_end = PIECES ? bg + 1 : min(p.B, (bg + 1) * p.per_bg);       // (an utterance a group where it is in pieces)
+    for (int b = PIECES ? bg : bg * p.per_bg; b < b_end; ++b) {
         const int len = valid_steps(p.lens, b, p.T), nv = (len + SEG - 1) / SEG;
         float carry[NC][NS];
+        const auto last_gradients = [&] {
 #pragma unroll
-        for (int k = 0; k < NC; ++k)
+            for (int k = 0; k < NC; ++k)
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                const int c = l.c0 + k, n = l.ng * NS + j;
-                carry[k][j] = p.dlast && c < l.cend && n < p.N ? p.dlast[((int64_t)b * p.D + c) * p.N + n] : 0.f;
-            }
-        const int s0 = chunk * p.spc, s1 = min(nv, s0 + p.spc), end = min(p.T, (s0 + p.spc) * SEG);
-        if (s0 < nv)
-            for (int c = (nv - 1) / p.spc; c > chunk; --c) carry_over<NS>(p, l, b, c, A2, carry);
+                for (int j = 0; j < NS; ++j) {
+                    const int c = l.c0 + k, n = l.ng * NS + j;
+                    carry[k][j] = p.dlast && c < l.cend && n < p.N ? p.dlast[((int64_t)b * p.D + c) * p.N + n] : 0.f;
+                }
+        };
+        last_gradients();
+        const int s0 = PIECES ? chunk * p.spc : 0, s1 = PIECES ? min(nv, s0 + p.spc) : nv, end = PIECES ? min(p.T, (s0 + p.spc) * SEG) : p.T;
+        if (PIECES && s1 < nv)
+            carry_all<NS>(carry, [&](auto careful) { for (int c = (nv - 1) / p.spc; c > chunk; --c) carry_over<NS, decltype(careful)::value>(p, l, b, c, A2, carry); },
+                          last_gradients, [&] { last_gradients(); over_frames<T, NS, true>(dy, delta, cm, GATED ? z : View<const T>{}, p, l, b, s1 * SEG, len, A2, carry); });
         for (int t = max(nv, s0) * SEG + l.otp; t < end; t += TQ)
             if (l.ocv) {
                 du.row(b, t)[l.oc] = (T)0.f;
@@ -677,7 +744,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             turn ^= 1;
         }
-        if (p.dstate && chunk == 0)
+        if (p.dstate && (!PIECES || chunk == 0))
 #pragma unroll
             for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -920,21 +987,26 @@ ScanParams params(const adn_scan_args& a, const Plan& q) {
     return p;
 }
 
+// go(...) with every truth value as a type
+template <typename F, typename... Rest> void choose(const F& go, bool first, Rest... rest) {
+    if constexpr (sizeof...(rest) == 0) {
+        if (first) go(std::true_type{});
+        else go(std::false_type{});
+    } else {
+        if (first) choose([&](auto... t) { go(std::true_type{}, t...); }, rest...);
+        else choose([&](auto... t) { go(std::false_type{}, t...); }, rest...);
+    }
+}
+
 template <typename T, int NS> int forward(const adn_scan_args& a, const ScanParams& p, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.B * p.chunks * p.bpg * p.G));
     if (p.chunks > 1)
         hipLaunchKernelGGL((scan_local_kernel<T, NS, false, false>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), View<const T>{}, p);
-#define ADN_SCAN_GO(GATED, SAVE)                                                                                                                        \
-    hipLaunchKernelGGL((scan_forward_kernel<T, NS, GATED, SAVE>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
-                       cview<T>(a.z), view<T>(a.y), p)
-    if (a.z.data) {
-        if (p.ckpt) ADN_SCAN_GO(true, true);
-        else ADN_SCAN_GO(true, false);
-    } else {
-        if (p.ckpt) ADN_SCAN_GO(false, true);
-        else ADN_SCAN_GO(false, false);
-    }
-#undef ADN_SCAN_GO
+    const auto go = [&](auto gated, auto save, auto pieces) {
+        hipLaunchKernelGGL((scan_forward_kernel<T, NS, decltype(gated)::value, decltype(save)::value, decltype(pieces)::value>), grid, dim3(256), 0, s, cview<T>(a.u),
+                           cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), cview<T>(a.z), view<T>(a.y), p);
+    };
+    choose(go, a.z.data != nullptr, p.ckpt != nullptr, p.chunks > 1);
     ADN_HIP_CHECK(hipGetLastError());
     return ADN_OK;
 }
@@ -945,15 +1017,14 @@ template <typename T, int NS> int backward(const adn_scan_args& a, const ScanPar
         if (a.z.data) hipLaunchKernelGGL((scan_local_kernel<T, NS, true, true>), grid, dim3(256), 0, s, cview<T>(a.dy), cview<T>(a.delta), cview<T>(a.c), cview<T>(a.z), p);
         else hipLaunchKernelGGL((scan_local_kernel<T, NS, true, false>), grid, dim3(256), 0, s, cview<T>(a.dy), cview<T>(a.delta), cview<T>(a.c), View<const T>{}, p);
     }
-#define ADN_SCAN_GO(GATED)                                                                                                                          \
-    hipLaunchKernelGGL((scan_backward_kernel<T, NS, GATED>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta), cview<T>(a.b), cview<T>(a.c), \
-                       cview<T>(a.z), cview<T>(a.dy), view<T>(a.du), view<T>(a.ddelta), view<T>(a.dz), p)
+    const auto go = [&](auto gated, auto pieces) {
+        hipLaunchKernelGGL((scan_backward_kernel<T, NS, decltype(gated)::value, decltype(pieces)::value>), grid, dim3(256), 0, s, cview<T>(a.u), cview<T>(a.delta),
+                           cview<T>(a.b), cview<T>(a.c), cview<T>(a.z), cview<T>(a.dy), view<T>(a.du), view<T>(a.ddelta), view<T>(a.dz), p);
+    };
     if (p.B > 0) {
-        if (a.z.data) ADN_SCAN_GO(true);
-        else ADN_SCAN_GO(false);
+        choose(go, a.z.data != nullptr, p.chunks > 1);
         ADN_HIP_CHECK(hipGetLastError());
     }
-#undef ADN_SCAN_GO
     const int64_t bc = (int64_t)p.B * p.T * p.G * p.N * 2, rest = (int64_t)p.D * (p.N + 2);
     const int64_t nb_bc = (bc + 255) / 256;
     hipLaunchKernelGGL((scan_reduce_kernel<T, NS>), dim3((unsigned)(nb_bc + (rest + 31) / 32)), dim3(256), 0, s, static_cast<T*>(a.dB), static_cast<T*>(a.dC),

@@ -230,8 +230,7 @@ def selective_scan_forward(u, delta, A, Bm, Cm, D=None, z=None, delta_bias=None,
         dt = softplus(delta + delta_bias)          (softplus=False: the sum itself)
         h  = exp(dt A) h + dt u Bm;   y = sum_n h Cm + D u;   y *= z sigmoid(z)  if z is given
 
-    A scan may grow, as long as ``exp(dt A)`` of a frame and the states are float32 numbers (``include/adenet.h`` says what is lost where
-    the input cancels a growth past 2^127).
+    A scan may grow (``A`` > 0, or steps below 0), as long as ``exp(dt A)`` of a frame and the states are float32 numbers.
     ``state`` (batch, channels, states), float32: the state to start from (None: zeros).  Returns ``(y, state, saved)``: the state behind
     the last valid frame and, with ``save=True``, what ``selective_scan_backward`` needs (else None)."""
     _first("u", u, (3,))

@@ -188,3 +188,46 @@ def test_refusals_of_bad_statistics_and_of_empty_tensors_with_a_dimension_of_2_3
     for fn in (S.layer_norm_forward, lambda v: S.causal_conv_forward(v, one), lambda v: S.selective_scan_forward(v, v, -one, v, v)):
         with pytest.raises(ValueError, match=r"2\^31"):
             fn(far)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("N,D,G", GROWTH)
+def test_an_input_that_cancels_a_growth_past_float32(S, dtype, N, D, G):
+    """The first utterance's state of 1 is cancelled exactly by its input in frame 64, then the scan grows by e^120: a piece of the time
+    axis alone ends in infinities, frame by frame there are zeros.  On the way back the gradient of the last state meets its opposite in
+    frame 191, behind a growth by e^120.  The second utterance is an ordinary one."""
+    torch = _torch()
+    rng = np.random.default_rng([45, N, D])
+    B, T, tiny = 2, 256, 2.0 ** -30
+    assert S._lib.load().adn_op_selective_scan_workspace(B, T, D, N, G, 0) > 0      # pieces
+    delta = np.full((B, T, D), tiny)
+    delta[0, 65:97] = delta[0, 159:191] = 3.75
+    delta[1] = rng.uniform(0.01, 0.02, (T, D))
+    u, dy = rng.normal(size=(B, T, D)), rng.normal(size=(B, T, D))
+    bm, cm = rng.normal(size=(B, T, G, N)), rng.normal(size=(B, T, G, N))
+    u[0], dy[0], bm[0], cm[0] = 0, 0, 1, 1
+    u[0, 64] = -1 / tiny
+    dy[0, 191] = -1
+    state, dlast = rng.normal(size=(B, D, N)), rng.normal(size=(B, D, N))
+    state[0] = dlast[0] = 1
+    (_, u), (_, delta), (_, bm), (_, cm), (_, dy) = (_dev(v, dtype) for v in (u, delta, bm, cm, dy))
+    (_, A), (_, state), (_, dlast) = _dev(np.ones((D, N))), _dev(state), _dev(dlast)
+    y, last, saved = S.selective_scan_forward(u, delta, A, bm, cm, state=state, softplus=False, save=True)
+    h = state.clone()
+    for t in range(T):
+        yt = S.selective_scan_step(u[:, t], delta[:, t], A, bm[:, t], cm[:, t], h, softplus=False)
+        assert torch.equal(y[0, t], yt[0]), t
+    assert torch.isfinite(h).all() and not h[0].any() and torch.equal(last[0], h[0])
+    assert torch.isfinite(y).all() and y[0, :64].any() and not y[0, 64:].any()
+    g = S.selective_scan_backward(dy, u, delta, A, bm, cm, saved, state=state, softplus=False, dlast=dlast)
+    assert not g["dstate"][0].any() and not g["du"][0, :192].any() and not g["ddelta"][0, :192].any()
+    # dh = 1 (to the rounding of 64 factors of 1 + 2^-30) behind frame 191: du = dt sum_n dh B, ddelta = A sum_n dh h = 0
+    assert ((g["du"][0, 192:].double() / (tiny * N) - 1).abs() <= (2.0 ** -8 if dtype == "bfloat16" else 64 * 2.0 ** -23)).all() and not g["ddelta"][0, 192:].any()
+    assert all(torch.isfinite(v).all() for v in g.values() if v is not None)
+    # the other utterance as if alone
+    one = [v[1:].contiguous() for v in (u, delta, bm, cm, dy)]
+    y1, last1, saved1 = S.selective_scan_forward(one[0], one[1], A, one[2], one[3], state=state[1:], softplus=False, save=True)
+    g1 = S.selective_scan_backward(one[4], one[0], one[1], A, one[2], one[3], saved1, state=state[1:], softplus=False, dlast=dlast[1:])
+    assert torch.equal(y[1:], y1) and torch.equal(last[1:], last1)
+    for name in ("du", "ddelta", "dB", "dC", "dstate"):
+        assert torch.equal(g[name][1:], g1[name]), name
