@@ -176,7 +176,10 @@ template <int P> __device__ __forceinline__ int64_t ckpt_at(const ScanParams& p,
 template <int P> __device__ __forceinline__ int64_t local_at(const ScanParams& p, int b, int chunk, int ctile) {
     return (((int64_t)b * p.chunks + chunk) * p.ctiles + ctile) * 64 * P;
 }
-// x (a state, or a state's gradient) carried over a piece: x = what the piece alone leaves + exp(A sum dt) x
+// x (a state, or a state's gradient) carried over a piece: x = what the piece alone leaves + exp(A sum dt) x.  The factor may be no float32
+// number where the product is -- the state shrinks from a large one, or grows from a tiny one -- so it is applied in halves: down to
+// 2^-252 and up to 2^256.  CAREFUL: in thirds of at most 2^127, for what a growth past that makes of a state of zero (NaN in halves)
+// or of a denormal one
 template <int NS, bool CAREFUL>
 __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>& l, int b, int chunk, const float (&A2)[Place<NS>::NC][NS],
                                            float (&x)[Place<NS>::NC][NS]) {
@@ -188,15 +191,12 @@ __device__ __forceinline__ void carry_over(const ScanParams& p, const Place<NS>&
     for (int m = 0; m < P / 4; ++m) load_vec<float, 4>(src + m * 256, v + m * 4);
     load_vec<float, NC>(ds, d);
 #pragma unroll
+    for (int k = 0; k < NC; ++k) d[k] *= CAREFUL ? 1.f / 3.f : 0.5f;
+#pragma unroll
     for (int m = 0; m < P; ++m) {
-        const float e = d[m / NS] * A2[m / NS][m % NS];
-        if (CAREFUL) {
-            // a scan that grows (A > 0, or steps below 0) may take a tiny state through more than 2^128, and what it grows by on a zero is
-            // no infinity: a third of the exponent at a time, 127 of them at most (more is past any pair of numbers)
-            const float f = __builtin_amdgcn_exp2f(fminf(e * (1.f / 3.f), 127.f));
-            x[m / NS][m % NS] = fmaf(x[m / NS][m % NS] * f * f, f, v[m]);
-        } else
-            x[m / NS][m % NS] = fmaf(__builtin_amdgcn_exp2f(e), x[m / NS][m % NS], v[m]);
+        float& s = x[m / NS][m % NS];
+        const float e = d[m / NS] * A2[m / NS][m % NS], f = __builtin_amdgcn_exp2f(CAREFUL ? fminf(e, 127.f) : e);
+        s = fmaf(CAREFUL ? s * f * f : s * f, f, v[m]);
     }
 }
 template <int NC, int NS> __device__ __forceinline__ bool all_finite(const float (&x)[NC][NS]) {

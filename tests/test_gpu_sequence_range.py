@@ -231,3 +231,27 @@ def test_an_input_that_cancels_a_growth_past_float32(S, dtype, N, D, G):
     assert torch.equal(y[1:], y1) and torch.equal(last[1:], last1)
     for name in ("du", "ddelta", "dB", "dC", "dstate"):
         assert torch.equal(g[name][1:], g1[name]), name
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("N,D,G", GROWTH)
+def test_a_scan_that_shrinks_below_float32_in_one_piece_and_grows_back_in_another(S, dtype, N, D, G):
+    """States of 1e12 shrink by e^-100 within 32 frames, to 4e-32, and grow back later; the gradient of the last state the same on the way
+    back (from 1e-10 to 3e33 to 1e-10).  Every h and dh is a float32 number, e^-100 (and e^100) is none."""
+    rng = np.random.default_rng([46, N, D])
+    B, T = 2, 256
+    assert S._lib.load().adn_op_selective_scan_workspace(B, T, D, N, G, 0) > 0      # pieces
+    delta = np.full((B, T, D), 2.0 ** -12)
+    delta[0, 64:96], delta[0, 160:192] = 3.125, -3.125
+    delta[1] = rng.uniform(0.01, 0.02, (T, D))
+    u, dy = rng.normal(size=(B, T, D)), rng.normal(size=(B, T, D))
+    u[0, :192] = 0
+    dy[0] = 0
+    state, dlast = rng.normal(size=(B, D, N)), rng.normal(size=(B, D, N))
+    state[0], dlast[0] = 1e12 * np.abs(state[0]), 1e-10 * np.abs(dlast[0])
+    v, t = _both(dict(u=_dev(u, dtype), delta=_dev(delta, dtype), A=_dev(np.full((D, N), -1.0)), Bm=_dev(rng.normal(size=(B, T, G, N)), dtype),
+                      Cm=_dev(rng.normal(size=(B, T, G, N)), dtype), D=_dev(rng.normal(size=D)), state=_dev(state)))
+    want = _check_scan(S, v, t, _dev(dy, dtype), _dev(dlast), [T, T - 3], dtype, False)
+    for name in ("state", "dstate"):
+        assert (np.abs(want[name].e[0] / want[name].v[0]) < 1e-2).mean() > 0.9, name
+    assert (np.abs(want["state"].v[0] / v["state"][0] - 1) < 0.2).all()
