@@ -8,7 +8,7 @@
 // with the taps' window in registers, so a run costs K - 1 frames beyond its own (backward: K - 1 on each side, the second of them
 // for the dpre behind the run's end; those come from the caches).  The backward pass adds dw and dbias in registers over all the
 // runs of a workgroup, which leaves one partial row; sum_parts adds them in a fixed order.  4 x 4096 x 4096 bfloat16, 4 taps: forward
-// 51 us (5.3 TB/s), backward 98 us (4.1 TB/s); 520 utterances of 12 to 40 frames x 1000: 23 and 36 us, where the one chunk of frames
+// 50 us (5.4 TB/s), backward 97 us (4.1 TB/s); 520 utterances of 12 to 40 frames x 1000: 23 and 37 us, where the one chunk of frames
 // in flight per wave leaves the loads' latency in sight.
 // Vectors are read at any element's address, and where V does not divide C the last lane's channels begin at C - V: it computes some of
 // its neighbour's again and writes the same values.  float32, 5 taps, 373 utterances of up to 2120 frames x 105: forward 121 us, with one channel

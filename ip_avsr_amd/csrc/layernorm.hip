@@ -8,7 +8,7 @@
 // per thread, forward on one wave 32: more registers per thread cost the waves that hide the loads).  The workgroups are persistent:
 // gamma and beta stay in registers over all their rows, the next row's loads are in flight during a row's sums, and the backward pass adds dgamma / dbeta there too, leaves one partial row per workgroup, and a
 // second launch adds those in a fixed order -- the same bits on every run.  32768 x 4096 bfloat16: forward 96 us (5.6 TB/s), backward
-// 171 us (4.7 TB/s) and 6 us for the partial rows; 13520 of 20800 x 1000 float32: 29, 35 and 5 us.  Narrow rows leave most of a wave
+// 169 us (4.8 TB/s) and 6 us for the partial rows; 13520 of 20800 x 1000 float32: 28, 35 and 5 us.  Narrow rows leave most of a wave
 // idle: 10^6 rows of 50 float32 take 261 and 395 us (the memory 80 and 120), its two 64-lane sums a row being the limit.
 // Frames at and behind lens[b] are padding: not read, zero in every result, absent from the sums.
 #include "seq_common.h"

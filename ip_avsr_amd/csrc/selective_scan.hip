@@ -22,7 +22,7 @@
 // rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
 // over all frames of a workgroup's utterances.  All sums run in a fixed order.
 // 8 x 2048 x 2048 x 16 bfloat16, gated: forward 285 us with what training keeps, 0.53 us per 10^6 (t, d, n) where the 8 slots take 0.20
-// (1024 waves, one per SIMD, the pipe 47 % busy: nothing covers a wave's own waits; with four per SIMD 0.33), backward 497 us (26 vector instructions a (t, d, n), the pipe 87 % busy) behind 131 us for the pieces alone.
+// (1024 waves, one per SIMD, the pipe 47 % busy: nothing covers a wave's own waits; with four per SIMD 0.33), backward 469 us (26 vector instructions a (t, d, n), the pipe 90 % busy) behind 131 us for the pieces alone.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
 #include <type_traits>
