@@ -404,7 +404,8 @@ typedef struct {
 } adn_seq;
 
 /* y = (x - mean) inv_std gamma + beta over the channels, inv_std = 1 / sqrt(var + eps); channels <= 16384.  gamma null: 1, beta
- * null: 0.  mean and inv_std (float32 [B][T]) are results of the forward pass and inputs of the backward pass. */
+ * null: 0.  mean and inv_std (float32 [B][T]) are results of the forward pass and inputs of the backward pass.  The sums of a row and of
+ * its squared deviations are float32 numbers too: rows that spread past about 1e17 are outside. */
 typedef struct {
     int32_t dtype, batch, steps, channels;
     float eps;

@@ -22,7 +22,8 @@
 // rotations), over the workgroup's waves in LDS and over workgroups by a second launch; dA, dD and the bias' gradient stay in registers
 // over all frames of a workgroup's utterances.  All sums run in a fixed order.
 // 8 x 2048 x 2048 x 16 bfloat16, gated: forward 285 us with what training keeps, 0.53 us per 10^6 (t, d, n) where the 8 slots take 0.20
-// (1024 waves, one per SIMD, the pipe 47 % busy: nothing covers a wave's own waits; with four per SIMD 0.33), backward 469 us (26 vector instructions a (t, d, n), the pipe 90 % busy) behind 131 us for the pieces alone.
+// (1024 waves, one per SIMD, the pipe 47 % busy: nothing covers a wave's own waits; with four per SIMD 0.33), backward 469 us (26 vector
+// instructions a (t, d, n), the pipe 90 % busy) behind 131 us for the pieces alone.
 // Frames at and behind lens[b] are padding: not read, zero in y and the frame gradients; the state passes them unchanged.
 #include "seq_common.h"
 #include <type_traits>
@@ -367,7 +368,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     if (l.otp == 0) p.dsum[(((int64_t)b * p.chunks + chunk) * p.ctiles + l.ctile) * WC + l.cl * NC + l.ng] = total;
 }
 
-// PIECES: the time axis is split (an unsplit one has no carries, and no registers for them)
+// PIECES: the time axis is split.  The unsplit kernels hold no registers for the carries, and a split one walks one utterance backward
+// (520 x 40 x 1000 x 16, unsplit: backward 295 us, as one kernel for both 307; 1 x 8192 x 2048 x 16, split: 296 and 318)
 template <typename T, int NS, bool GATED, bool SAVE, bool PIECES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) void scan_forward_kernel(View<const T> u, View<const T> delta, View<const T> bm, View<const T> cm, View<const T> z,
                                                            View<T> y, ScanParams p) {

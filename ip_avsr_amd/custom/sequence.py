@@ -89,7 +89,8 @@ def _floats(n, x):
 def layer_norm_forward(x, gamma=None, beta=None, lens=None, eps=1e-5):
     """Layer norm over the last dimension of ``x`` (rows, channels) or (batch, time, channels), at most 16384 channels:
     ``(x - mean) inv_std gamma + beta`` with ``inv_std = 1 / sqrt(var + eps)``.  Returns ``(y, mean, inv_std)``; the statistics
-    (float32, the shape of the rows) are what the backward pass needs."""
+    (float32, the shape of the rows) are what the backward pass needs.  The sum of a row's squared deviations has to be a float32 number
+    (rows that spread past about 1e17 are outside)."""
     _first("x", x, (2, 3))
     if x.dim() == 2:
         y, mean, inv = layer_norm_forward(x[None], gamma, beta, lens, eps)
