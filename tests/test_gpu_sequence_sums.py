@@ -74,15 +74,11 @@ SCAN = [((2500, 3, 20), 4, 1), ((1500, 2, 70), 16, 2), ((300, 9, 300), 8, 1), ((
         ((2, 150, 150), 16, 1), ((1, 140, 300), 16, 2), ((2, 150, 130), 31, 1), ((2, 261, 300), 5, 1), ((1, 200, 600), 3, 2)]
 
 
-@pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape,N,G", SCAN, ids=str)
-def test_selective_scan_exactly(S, dtype, shape, N, G):
+def _scan_exactly(S, dtype, shape, N, G):
     rng = np.random.default_rng([63, *shape, N, G])
     B, T, D = shape
     lens = rng.integers(0, T + 1, size=B)
     lens[0] = T
-    if T >= 128:
-        assert S._lib.load().adn_op_selective_scan_workspace(B, T, D, N, G, 0) > 0      # pieces
     v = dict(u=_ints(rng, B, T, D, most=1), dt=rng.integers(0, 3, size=shape), Bm=_ints(rng, B, T, G, N, most=1), Cm=_ints(rng, B, T, G, N, most=1), D=_ints(rng, D),
              state=_ints(rng, B, D, N, most=2), dy=_ints(rng, B, T, D, most=1), dlast=_ints(rng, B, D, N, most=2))
     want = I.scan(lens=lens, **v)
@@ -95,6 +91,22 @@ def test_selective_scan_exactly(S, dtype, shape, N, G):
     for name, got in dict(g, y=y, state=state).items():
         if name != "dz":
             _equal(name, got, want[name])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,N,G", SCAN, ids=str)
+def test_selective_scan_exactly(S, dtype, shape, N, G):
+    assert shape[1] < 128 or S._lib.load().adn_op_selective_scan_workspace(*shape, N, G, 0) > 0      # pieces
+    _scan_exactly(S, dtype, shape, N, G)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,G,N", [(49, 130, 16, 4), (50, 140, 16, 17)])
+def test_a_backward_pass_in_pieces_behind_a_forward_pass_in_one(S, dtype, B, T, G, N):
+    """Rows enough for the forward pass to take the time axis whole (more than 768 waves, here one a group) and not for the backward pass."""
+    need = S._lib.load().adn_op_selective_scan_workspace
+    assert need(B, T, G, N, G, 0) == 0 and need(48, T, G, N, G, 0) > 0
+    _scan_exactly(S, dtype, (B, T, G), N, G)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -118,3 +130,44 @@ def test_pieces_of_the_time_axis_over_several_workgroups(S, dtype, gated, carrie
         _near(name, g[name], want[name], dtype)
     for name in ("dA", "dD", "ddelta_bias") + (("dstate",) if carried else ()):
         _near(name, g[name], want[name])
+
+
+def test_pieces_of_the_time_axis_captured_into_a_graph(S):
+    """Forward and backward with a split time axis, captured, replayed on new inputs with eager work between; and two such graphs in turn."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(64)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")               # noqa: E731
+    sets = []
+    for B, T, D, N in ((2, 200, 130, 16), (1, 260, 70, 5)):
+        assert S._lib.load().adn_op_selective_scan_workspace(B, T, D, N, 1, 0) > 0
+        lens = torch.randint(1, T + 1, (B,), dtype=torch.int32, generator=g, device="cuda")
+        sets.append(dict(u=rn(B, T, D), delta=rn(B, T, D), A=-torch.exp(rn(D, N)), Bm=rn(B, T, N), Cm=rn(B, T, N), D=rn(D), z=rn(B, T, D), state=rn(B, D, N), lens=lens))
+
+    def passes(t):
+        y, state, saved = S.selective_scan_forward(save=True, **t)
+        out = S.selective_scan_backward(t["z"], saved=saved, dlast=t["state"], **t)
+        return [y, state] + [out[k] for k in sorted(out)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for t in sets:
+            passes(t)
+    side.synchronize()
+    graphs, outs = [], []
+    for t in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(passes(t))
+        graphs.append(graph)
+    for turn in range(4):
+        for k, t in enumerate(sets):
+            for name in ("u", "delta", "Bm", "z"):
+                t[name].copy_(rn(*t[name].shape))
+            want = passes(t)
+            for o in outs[k]:
+                o.zero_()
+            graphs[k].replay()
+            if turn % 2:
+                passes(sets[1 - k])
+            torch.cuda.synchronize()
+            for got, v in zip(outs[k], want):
+                assert torch.equal(got, v)
